@@ -50,6 +50,10 @@ extern "C" {
 #define KGE_TIE_BEST 1
 #define KGE_TIE_WORST 2
 
+#define KGE_DT_F32 0  /* element types of the post-training operators below */
+#define KGE_DT_BF16 1
+#define KGE_DT_F16 2
+
 #define KGE_ERR_ARG 1001     /* invalid argument (shape, enum, null pointer) */
 #define KGE_ERR_ALIGN 1002   /* pointer / leading dimension alignment        */
 #define KGE_ERR_NOGPU 1003   /* no gfx950 device visible                      */
@@ -578,6 +582,48 @@ int kge_rank_rows_codes(const void* codes, int64_t ldc, int64_t n_a, int64_t n_b
  * kge_rank_rows).  No counterpart in the reference, which ranks exact fp32 scores
  * (entity_ranking.py:469-529). */
 int kge_row_norm_max(const float* t, int64_t ldt, int64_t m, int d, float* out, void* stream);
+
+/* ---- losses on the log-probability of one label per score row -----------------------------------
+ * Post-training of a trained model (no counterpart in the reference): score rows S [n, m] of type
+ * dtype (KGE_DT_*), row stride lds in elements (any), labels[i] in [0, m) or -1 (the row carries
+ * nothing: log-probability 0, zero gradient, not read).  x = S / temperature,
+ *   logp[i] = x[i, labels[i]] - logsumexp_j x[i, j]
+ * A label outside [-1, m) gives NaN.  Needs a workspace of kge_label_ws_size bytes, 16-B aligned,
+ * of this call's own (calls that overlap on the device must not share one); pairs: 0 except for
+ * kge_preference_loss.  stats [n, 2] and coef [n] are what kge_label_grad takes; where a call may
+ * leave them out they may be null. */
+int64_t kge_label_ws_size(int64_t n, int64_t m, int dtype, int64_t pairs);
+
+int kge_label_logprobs(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
+                       double temperature, float* logp, float* stats, void* ws, int64_t ws_bytes, void* stream);
+
+/* g[i, j] = gscale[0] coef[i] / temperature ([j == labels[i]] - softmax_j x[i, j]) in S's type: the
+ * gradient of sum_i coef[i] logp[i].  gscale: device scalar or null (1).  g may be s (same stride). */
+int kge_label_grad(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
+                   double temperature, const float* stats, const float* coef, const float* gscale, void* g,
+                   int64_t ldg, void* stream);
+
+/* Clipped policy loss with a KL term, r_i = exp(logp_i - old_logp_i), d_i = ref_logp_i - logp_i:
+ *   loss[0] = scale sum_i weights_i (-min(r_i A_i, clip(r_i, 1 - clip_low, 1 + clip_high) A_i)
+ *                                    + kl (exp(d_i) - d_i - 1))
+ * ref_logp null: no KL term; weights null: 1.  g non-null: the gradient with respect to S from the
+ * same call (may be s, same stride: in place).  stats / coef: for a later kge_label_grad, or null. */
+int kge_policy_loss(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
+                    const float* advantages, const float* old_logp, const float* ref_logp, const float* weights,
+                    double clip_low, double clip_high, double kl, double temperature, double scale, float* loss,
+                    float* logp, float* stats, float* coef, void* g, int64_t ldg, void* ws, int64_t ws_bytes,
+                    void* stream);
+
+/* Preference loss on pairs of sequences: sequence q is the rows [seq_ptr[q], seq_ptr[q + 1])
+ * (seq_ptr [2 pairs + 1], ascending; bounds are clamped to [0, n]), pair k prefers sequence 2 k
+ * to 2 k + 1.  pi_q = sum (average: mean) of logp over the labelled rows of q (0 without any),
+ *   z_k = beta ((pi_2k - ref_logp_2k) - (pi_2k+1 - ref_logp_2k+1))          (ref_logp null: 0)
+ *   loss[0] = scale sum_k -((1 - smoothing) log sigma(z_k) + smoothing log sigma(-z_k))
+ * seq_logp [2 pairs] = pi; logp [n].  Rows of no sequence get a zero gradient.  g, stats, coef as above. */
+int kge_preference_loss(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
+                        const int64_t* seq_ptr, int64_t pairs, const float* ref_logp, double beta, double smoothing,
+                        int average, double temperature, double scale, float* loss, float* seq_logp, float* logp,
+                        float* stats, float* coef, void* g, int64_t ldg, void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,12 +28,14 @@ DIR_SP, DIR_PO = 0, 1
 PREC_FP32, PREC_BF16X3 = 0, 1
 DIST_L1, DIST_L2, DIST_ROT_L1, DIST_ROT_L2 = range(4)
 TIE = {"rounded_mean_rank": 0, "best_rank": 1, "worst_rank": 2}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # KGE_DT_*
 PRECISIONS = {"fp32": PREC_FP32, "bf16x3": PREC_BF16X3}
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 SIGNATURES = {
     "kge_version": ([], _I),
@@ -109,6 +111,13 @@ SIGNATURES = {
     "kge_softmax_grad": ([_P, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _I64, _P], _I),
     "kge_softmax_grad_planes": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _I64, _P], _I),
     "kge_grad_planes_chunks": ([_I64], _I64),
+    "kge_label_ws_size": ([_I64, _I64, _I, _I64], _I64),
+    "kge_label_logprobs": ([_P, _I, _I64, _I64, _I64, _P, _D, _P, _P, _P, _I64, _P], _I),
+    "kge_label_grad": ([_P, _I, _I64, _I64, _I64, _P, _D, _P, _P, _P, _P, _I64, _P], _I),
+    "kge_policy_loss": ([_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _P, _P, _P, _P, _I64,
+                         _P, _I64, _P], _I),
+    "kge_preference_loss": ([_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _D, _D, _I, _D, _D, _P, _P, _P, _P, _P, _P,
+                             _I64, _P, _I64, _P], _I),
     "kge_bce_grad_planes": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _F, _F, _P, _I64, _P, _P], _I),
 }
 

@@ -821,3 +821,8 @@ def score_spo_emb(kind: int, l_norm: float, s_emb, p_emb, o_emb) -> torch.Tensor
     so = torch.cat((s_emb, o_emb), 0)
     ar = torch.arange(n, device=p_emb.device)
     return score_spo(kind, l_norm, so, ar, p_emb, ar, ar + n)
+
+
+# Post-training operators: losses on sampled or preferred answers
+from .label_losses import (label_logprobs, policy_loss, policy_loss_grad, preference_loss,  # noqa: E402, F401
+                           preference_loss_grad)
