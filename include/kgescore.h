@@ -625,6 +625,45 @@ int kge_preference_loss(const void* s, int dtype, int64_t lds, int64_t n, int64_
                         int average, double temperature, double scale, float* loss, float* seq_logp, float* logp,
                         float* stats, float* coef, void* g, int64_t ldg, void* ws, int64_t ws_bytes, void* stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection -------------------------------
+ * Post-training of a trained model (no counterpart in the reference).  Types KGE_DT_F32 and KGE_DT_BF16;
+ * requests x [n, d], shared w [m, d], adapters a [k, r, d] and b [k, m, r] (contiguous), ids[i] in
+ * [0, k) or -1 (no adapter); r <= 1024.  rp = r rounded up to 16:
+ *   h_i = scales_t A_t x_i,  y_i = W x_i + B_t h_i,  u_i = scales_t B_t^T dy_i,  dx_i = W^T dy_i + A_t^T u_i,
+ *   dA_t = sum_{i in t} u_i x_i^T,  dB_t = sum_{i in t} dy_i h_i^T        (zeros for an adapter without rows)
+ * An id outside [-1, k) poisons its own row (NaN). */
+
+/* The rows in the order of their adapters: perm [n] (sorted position -> row), sid [n] (its adapter; k: none,
+ * k + 1: out of range), start [k + 3] (first position of each group).  Stable, no atomics. */
+int kge_adapter_plan(const int64_t* ids, int64_t n, int64_t k, int32_t* perm, int32_t* sid, int32_t* start,
+                     void* stream);
+
+/* out[i, 0 .. rp) = scales_t F_t v_perm[i] for the sorted rows i of an adapter (other rows undefined), v [n, cols].
+ * F_t as [r, cols] (f_by_rank 1: A for h) or [cols, r] (f_by_rank 0: B for u); scales null: 1.
+ * out: kge_adapter_shrink_rows(...) rows of rp floats, 16-B aligned, of which the first n are the result
+ * (the others hold partial sums of the split columns). */
+int64_t kge_adapter_shrink_rows(int64_t n, int64_t cols, int64_t k, int64_t r);
+int kge_adapter_shrink(const void* v, int dtype, int64_t ldv, int64_t n, int64_t cols, const void* f, int f_by_rank,
+                       int64_t k, int64_t r, const float* scales, const int32_t* perm, const int32_t* start,
+                       float* out, int64_t out_rows, void* stream);
+
+/* y[perm[i], :] = W x_perm[i] + F_t h[i], F_t as [m, r] (f_by_rank 0: B) or [r, m] (f_by_rank 1: A, for dx from
+ * dy, W transposed and u).  h [n, rp] as kge_adapter_shrink leaves it. */
+int kge_adapter_project(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
+                        int64_t m, const void* f, int f_by_rank, int64_t k, int64_t r, const float* h,
+                        const int32_t* perm, const int32_t* sid, void* y, int64_t ldy, void* stream);
+
+/* out_t = sum over the sorted rows i of adapter t of h[i, q] v[perm[i], c], as [cols, r] (out_by_rank 0: dB from dy
+ * and h) or [r, cols] (out_by_rank 1: dA from x and u).  ws: kge_adapter_grads_ws_size floats (may be 0). */
+int64_t kge_adapter_grads_ws_size(int64_t n, int64_t cols, int64_t k, int64_t r, int dtype);
+int kge_adapter_grads(const void* v, int dtype, int64_t ldv, int64_t n, int64_t cols, const float* h, int64_t k,
+                      int64_t r, const int32_t* perm, const int32_t* start, void* out, int out_by_rank, float* ws,
+                      int64_t ws_elems, void* stream);
+
+/* dst [cols, rows] = src [rows, cols] transposed (KGE_DT_F32 / KGE_DT_BF16): W^T for dx */
+int kge_transpose(const void* src, int dtype, int64_t lds, int64_t rows, int64_t cols, void* dst, int64_t ldd,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

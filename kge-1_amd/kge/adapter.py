@@ -1,0 +1,188 @@
+"""Low-rank adapters of many requests at once beside a shared projection (csrc/adapter.hip; no
+counterpart in the reference): one frozen table -- the entity table of a trained model, or any
+[m, d] map -- serves many clients, domains or relations, each with a small correction of its own.
+
+    y_i = W x_i + scales_t B_t (A_t x_i),   t = ids[i]             (t = -1: no adapter)
+
+``adapted_projection`` is the operator, differentiable in x, a and b (W stays frozen);
+``LowRankAdapters`` holds the parameters; ``KgeModel.score_sp_adapted`` / ``score_po_adapted`` score
+queries against all entities with it.  fp32 tables use the fp32 matrix instruction, bf16 tables the bf16 one;
+sums are fp32 in both, results are rounded once.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib as L
+from .label_losses import _capturing, on_device_of
+
+MAX_RANK = 1024
+
+
+def _matrix(t: torch.Tensor, what: str) -> torch.Tensor:
+    """[rows, cols] with unit column stride and rows that do not overlap."""
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """[rows, cols] whose rows start on 16 bytes."""
+    per = 16 // like.element_size()
+    ld = (cols + per - 1) // per * per
+    buf = torch.empty(rows, ld, device=like.device, dtype=like.dtype)
+    return buf if ld == cols else buf[:, :cols]
+
+
+class _Plan:
+    """The rows of a batch in the order of their adapters."""
+
+    def __init__(self, ids: torch.Tensor, k: int):
+        n = ids.numel()
+        buf = torch.empty(2 * n + k + 3, device=ids.device, dtype=torch.int32)
+        self.perm, self.sid, self.start = buf[:n], buf[n:2 * n], buf[2 * n:]
+        L._check(L.lib().kge_adapter_plan(L.ptr(ids), n, k, L.ptr(self.perm), L.ptr(self.sid), L.ptr(self.start),
+                                          L.stream()), "kge_adapter_plan")
+
+    @staticmethod
+    def of(tensors):
+        plan = object.__new__(_Plan)
+        plan.perm, plan.sid, plan.start = tensors
+        return plan
+
+
+def _shrink(v, f, by_rank, k, r, scales, plan):
+    n, cols = v.shape
+    rows = L.lib().kge_adapter_shrink_rows(n, cols, k, r)
+    out = torch.empty(rows, (r + 15) // 16 * 16, device=v.device, dtype=torch.float32)
+    L._check(L.lib().kge_adapter_shrink(L.ptr(v), L.DTYPES[v.dtype], _ld(v), n, cols, L.ptr(f), int(by_rank), k, r,
+                                        L.ptr(scales), L.ptr(plan.perm), L.ptr(plan.start), L.ptr(out), rows,
+                                        L.stream()), "kge_adapter_shrink")
+    return out
+
+
+def _project(x, w, f, by_rank, k, r, h, plan):
+    n, d = x.shape
+    m = w.shape[0]
+    y = _padded(n, m, x)
+    L._check(L.lib().kge_adapter_project(L.ptr(x), L.DTYPES[x.dtype], _ld(x), n, d, L.ptr(w), _ld(w), m, L.ptr(f),
+                                         int(by_rank), k, r, L.ptr(h), L.ptr(plan.perm), L.ptr(plan.sid), L.ptr(y),
+                                         _ld(y), L.stream()), "kge_adapter_project")
+    return y
+
+
+def _grads(v, h, k, r, plan, by_rank):
+    n, cols = v.shape
+    out = torch.empty((k, r, cols) if by_rank else (k, cols, r), device=v.device, dtype=v.dtype)
+    size = L.lib().kge_adapter_grads_ws_size(n, cols, k, r, L.DTYPES[v.dtype])
+    ws = torch.empty(size, device=v.device, dtype=torch.float32) if size > 0 else None
+    L._check(L.lib().kge_adapter_grads(L.ptr(v), L.DTYPES[v.dtype], _ld(v), n, cols, L.ptr(h), k, r, L.ptr(plan.perm),
+                                       L.ptr(plan.start), L.ptr(out), int(by_rank), L.ptr(ws), size, L.stream()),
+             "kge_adapter_grads")
+    return out
+
+
+def _transposed(w):
+    out = _padded(w.shape[1], w.shape[0], w)
+    L._check(L.lib().kge_transpose(L.ptr(w), L.DTYPES[w.dtype], _ld(w), w.shape[0], w.shape[1], L.ptr(out), _ld(out),
+                                   L.stream()), "kge_transpose")
+    return out
+
+
+class _AdaptedProjection(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, a, b, ids, scales):
+        k, r = a.shape[0], a.shape[1]
+        plan = _Plan(ids, k)
+        h = _shrink(x, a, True, k, r, scales, plan)
+        y = _project(x, w, b, False, k, r, h, plan)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(x, w, a, b, scales, h, plan.perm, plan.sid, plan.start)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, a, b, scales, h, *plan = ctx.saved_tensors
+        plan = _Plan.of(plan)
+        k, r = a.shape[0], a.shape[1]
+        dx = da = db = None
+        with on_device_of(x):
+            dy = _matrix(dy, "dy")
+            if ctx.needs_input_grad[0] or ctx.needs_input_grad[2]:
+                u = _shrink(dy, b, False, k, r, scales, plan)
+            if ctx.needs_input_grad[0]:
+                dx = _project(dy, _transposed(w), a, True, k, r, u, plan)
+            if ctx.needs_input_grad[2]:
+                da = _grads(x, u, k, r, plan, True)
+            if ctx.needs_input_grad[3]:
+                db = _grads(dy, h, k, r, plan, False)
+        return dx, None, da, db, None, None
+
+
+def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
+                       scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y [n, m]: y_i = w x_i + scales[t] b[t] (a[t] x_i) for t = ids[i], y_i = w x_i for ids[i] = -1.
+
+    x [n, d] requests in any order, w [m, d] shared and frozen (pass it detached), a [k, r, d] and
+    b [k, m, r] the adapters (ranks below r: padded with zeros), scales [k] (None: 1), all of one type, fp32
+    or bf16 (scales in any floating type, used in fp32).  Differentiable in x, a and b."""
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"x: expected float32 or bfloat16, got {x.dtype}")
+    for t, dim, what in ((x, 2, "x [n, d]"), (w, 2, "w [m, d]"), (a, 3, "a [k, r, d]"), (b, 3, "b [k, m, r]")):
+        if t.dim() != dim or t.dtype != x.dtype:
+            raise ValueError(f"{what}: expected {dim} dimensions of {x.dtype}, got {list(t.shape)} {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"{what}: on {t.device}, x is on {x.device}")
+    (n, d), m, (k, r) = x.shape, w.shape[0], a.shape[:2]
+    if w.shape[1] != d or a.shape[2] != d or tuple(b.shape) != (k, m, r):
+        raise ValueError(f"x {list(x.shape)}, w {list(w.shape)}, a {list(a.shape)}, b {list(b.shape)}: expected "
+                         "[n, d], [m, d], [k, r, d], [k, m, r]")
+    if min(d, m, k) < 1 or not 1 <= r <= MAX_RANK:
+        raise ValueError(f"d={d}, m={m}, k={k}, r={r}: expected at least 1 each, ranks up to {MAX_RANK}")
+    if w.requires_grad and torch.is_grad_enabled():
+        raise ValueError("w: the shared projection is frozen, pass it detached")
+    if ids.dim() != 1 or ids.numel() != n or ids.is_floating_point() or ids.dtype == torch.bool:
+        raise ValueError(f"ids: expected {n} integers, got {list(ids.shape)} {ids.dtype}")
+    if scales is not None:
+        if scales.dim() != 1 or scales.numel() != k or not scales.is_floating_point():
+            raise ValueError(f"scales: expected {k} floating point numbers, got {list(scales.shape)} {scales.dtype}")
+        if scales.requires_grad and torch.is_grad_enabled():
+            raise ValueError("scales: no gradient flows into them, pass them detached")
+        scales = scales.detach().to(torch.float32).contiguous()
+    for t, what in ((ids, "ids"), (scales, "scales")):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: on {t.device}, x is on {x.device}")
+    ids = L.idx64(ids)
+    if L.CHECK_INDEX and n > 0 and not _capturing():
+        lo, hi = int(ids.min()), int(ids.max())
+        if lo < -1 or hi >= k:
+            raise IndexError(f"adapter id: out of range [{lo}, {hi}] for {k} adapters (-1: none)")
+    L.require_device(x)
+    with on_device_of(x):
+        return _AdaptedProjection.apply(_matrix(x, "x"), _matrix(w, "w"), a.contiguous(), b.contiguous(), ids, scales)
+
+
+class LowRankAdapters(torch.nn.Module):
+    """k adapters of rank r beside a [num_out, num_in] projection: ``a`` starts as N(0, 1 / num_in), ``b``
+    as zeros, so that a new adapter changes nothing.  ``alpha``: scales = alpha / r."""
+
+    def __init__(self, num_adapters: int, rank: int, num_in: int, num_out: int, alpha: Optional[float] = None,
+                 device=None, dtype=torch.float32):
+        super().__init__()
+        if min(num_adapters, num_in, num_out) < 1 or not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"num_adapters={num_adapters}, rank={rank}, num_in={num_in}, num_out={num_out}: expected "
+                             f"at least 1 each, ranks up to {MAX_RANK}")
+        self.a = torch.nn.Parameter(torch.randn(num_adapters, rank, num_in, device=device).mul_(num_in ** -0.5).to(dtype))
+        self.b = torch.nn.Parameter(torch.zeros(num_adapters, num_out, rank, device=device, dtype=dtype))
+        scale = 1.0 if alpha is None else float(alpha) / rank
+        self.register_buffer("scales", torch.full((num_adapters,), scale, device=device, dtype=torch.float32))
+
+    def forward(self, x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+        return adapted_projection(x, w, self.a, self.b, ids, self.scales)

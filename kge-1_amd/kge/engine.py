@@ -826,3 +826,4 @@ def score_spo_emb(kind: int, l_norm: float, s_emb, p_emb, o_emb) -> torch.Tensor
 # Post-training operators: losses on sampled or preferred answers
 from .label_losses import (label_logprobs, policy_loss, policy_loss_grad, preference_loss,  # noqa: E402, F401
                            preference_loss_grad)
+from .adapter import adapted_projection  # noqa: E402, F401  (low-rank adapters beside a shared projection)

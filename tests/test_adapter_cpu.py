@@ -1,0 +1,66 @@
+"""Refusals of the adapted projection (kge/adapter.py): every check of an argument comes before the
+check of the device, so they are all reached with CPU tensors and no launch."""
+import pytest
+import torch
+
+from kge import _lib as L
+from kge import engine
+from kge.adapter import LowRankAdapters
+
+
+def _args(n=5, d=8, m=6, k=3, r=2, dtype=torch.float32):
+    return dict(x=torch.randn(n, d).to(dtype), w=torch.randn(m, d).to(dtype), a=torch.randn(k, r, d).to(dtype),
+                b=torch.randn(k, m, r).to(dtype), ids=torch.tensor([0, 2, -1, 1, 0][:n]), scales=torch.ones(k))
+
+
+def test_cpu_tensors_are_refused_after_the_arguments():
+    for dtype in (torch.float32, torch.bfloat16):
+        with pytest.raises(L.EngineError, match="MI355X"):
+            engine.adapted_projection(**_args(dtype=dtype))
+    with pytest.raises(L.EngineError, match="MI355X"):
+        LowRankAdapters(3, 2, 8, 6)(torch.zeros(5, 8), torch.zeros(6, 8), torch.zeros(5, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("change, what", [
+    (dict(x=torch.zeros(5, 8, dtype=torch.float16)), "x"), (dict(x=torch.zeros(5, 8, 1)), "x"),
+    (dict(w=torch.zeros(6, 8, dtype=torch.bfloat16)), "w"), (dict(w=torch.zeros(6, 9)), "w"),
+    (dict(w=torch.zeros(6, 8, requires_grad=True)), "frozen"), (dict(w=torch.zeros(0, 8), b=torch.zeros(3, 0, 2)), "m=0"),
+    (dict(a=torch.zeros(2, 8)), "a"), (dict(a=torch.zeros(3, 2, 7)), "a"), (dict(b=torch.zeros(3, 2, 6)), "b"),
+    (dict(b=torch.zeros(4, 6, 2)), "b"), (dict(a=torch.zeros(3, 0, 8), b=torch.zeros(3, 6, 0)), "r=0"),
+    (dict(a=torch.zeros(1, 1025, 8), b=torch.zeros(1, 6, 1025)), "r=1025"),
+    (dict(ids=torch.zeros(4, dtype=torch.int64)), "ids"), (dict(ids=torch.zeros(5)), "ids"),
+    (dict(ids=torch.zeros(5, 1, dtype=torch.int64)), "ids"), (dict(scales=torch.ones(2)), "scales"),
+    (dict(scales=torch.ones(3, dtype=torch.int64)), "scales"), (dict(scales=torch.ones(3, requires_grad=True)), "scales")])
+def test_arguments_refused(change, what):
+    with pytest.raises(ValueError, match=what):
+        engine.adapted_projection(**{**_args(), **change})
+
+
+@pytest.mark.parametrize("bad", [-2, 3])
+def test_ids_out_of_range_refused_under_index_checking(bad):
+    with pytest.raises(IndexError, match="adapter id"):
+        engine.adapted_projection(**{**_args(), "ids": torch.tensor([0, 1, bad, -1, 2])})
+
+
+@pytest.mark.parametrize("args", [(0, 2, 8, 6), (3, 0, 8, 6), (3, 1025, 8, 6), (3, 2, 0, 6), (3, 2, 8, 0)])
+def test_module_sizes_refused(args):
+    with pytest.raises(ValueError):
+        LowRankAdapters(*args)
+
+
+def test_a_new_adapter_changes_nothing_and_scales_follow_alpha():
+    mod = LowRankAdapters(3, 4, 8, 6, alpha=8.0)
+    assert (mod.b == 0).all() and (mod.scales == 2.0).all() and mod.a.shape == (3, 4, 8) and mod.b.shape == (3, 6, 4)
+    assert set(mod.state_dict()) == {"a", "b", "scales"}
+
+
+def test_c_entries_refuse_bad_shapes_without_a_device():
+    lib = L.lib()
+    assert lib.kge_adapter_plan(None, 4, 3, None, None, None, None) == 1001
+    assert lib.kge_adapter_shrink(None, 2, 8, 4, 8, None, 1, 3, 2, None, None, None, None, 0, None) == 1001
+    assert lib.kge_adapter_shrink(None, 0, 7, 4, 8, None, 1, 3, 2, None, None, None, None, 0, None) == 1001
+    assert lib.kge_adapter_project(None, 0, 8, 4, 8, None, 8, 6, None, 0, 3, 2, None, None, None, None, 6, None) == 1001
+    assert lib.kge_adapter_grads(None, 0, 8, 4, 8, None, 3, 2000, None, None, None, 0, None, 0, None) == 1001
+    assert lib.kge_adapter_grads_ws_size(4, 8, 3, 2, 2) == 0
+    assert lib.kge_transpose(None, 0, 8, 4, 8, None, 4, None) == 1001
+    assert lib.kge_transpose(None, 0, 8, 0, 8, None, 4, None) == 0
