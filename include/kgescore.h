@@ -607,7 +607,8 @@ int kge_label_grad(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, 
  *   loss[0] = scale sum_i weights_i (-min(r_i A_i, clip(r_i, 1 - clip_low, 1 + clip_high) A_i)
  *                                    + kl (exp(d_i) - d_i - 1))
  * ref_logp null: no KL term; weights null: 1.  g non-null: the gradient with respect to S from the
- * same call (may be s, same stride: in place).  stats / coef: for a later kge_label_grad, or null. */
+ * same call (may be s, same stride: in place); stats and coef are then null.  g null: stats / coef for a
+ * later kge_label_grad, or null. */
 int kge_policy_loss(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
                     const float* advantages, const float* old_logp, const float* ref_logp, const float* weights,
                     double clip_low, double clip_high, double kl, double temperature, double scale, float* loss,

@@ -45,20 +45,25 @@ def _score_rows(scores: torch.Tensor) -> torch.Tensor:
     """The score block with unit column stride and rows that do not overlap."""
     if scores.dtype not in L.DTYPES:
         raise ValueError(f"scores: expected float32, bfloat16 or float16, got {scores.dtype}")
-    if scores.dim() != 2 or scores.shape[1] < 1:
-        raise ValueError(f"scores: expected [n, m] with m >= 1, got {list(scores.shape)}")
-    n, m = scores.shape
+    shape = scores.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"scores: expected [n, m] with m >= 1, got {list(shape)}")
+    n, m = shape
     if (m > 1 and scores.stride(1) != 1) or (n > 1 and scores.stride(0) < m):
         scores = scores.contiguous()
     return scores
 
 
 def _ld(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+    n, m = x.shape
+    return x.stride(0) if n > 1 else m
 
 
 def _labels(labels: torch.Tensor, scores: torch.Tensor) -> torch.Tensor:
     n, m = scores.shape
+    if labels.dtype is torch.int64 and labels.shape == (n,) and labels.is_contiguous() and not L.CHECK_INDEX:
+        _same_device(labels, scores, "labels")
+        return labels
     if labels.dim() != 1 or labels.numel() != n:
         raise ValueError(f"labels: expected [{n}], got {list(labels.shape)}")
     if labels.is_floating_point() or labels.dtype == torch.bool:
@@ -73,7 +78,7 @@ def _labels(labels: torch.Tensor, scores: torch.Tensor) -> torch.Tensor:
 
 
 def _same_device(t: torch.Tensor, scores: torch.Tensor, what: str):
-    if t.device != scores.device:
+    if t.get_device() != scores.get_device():  # (-1: CPU)
         raise ValueError(f"{what}: on {t.device}, the scores are on {scores.device}")
 
 
@@ -81,6 +86,9 @@ def _vector(t: Optional[torch.Tensor], n: int, scores: torch.Tensor, what: str) 
     """A constant of n numbers as contiguous fp32 on the scores' device."""
     if t is None:
         return None
+    if (t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous() and not t.requires_grad
+            and t.get_device() == scores.get_device()):
+        return t
     if t.dim() != 1 or t.numel() != n:
         raise ValueError(f"{what}: expected [{n}], got {list(t.shape)}")
     if t.requires_grad and torch.is_grad_enabled():

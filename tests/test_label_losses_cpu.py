@@ -109,9 +109,10 @@ def test_c_entries_refuse_bad_shapes_without_a_device():
 
 @pytest.mark.parametrize("n, m, pairs", [(1, 7, 0), (3, 100000, 500), (2047, 14541, 2048), (2049, 14541, 1)])
 def test_workspace_covers_parts_rows_and_losses(n, m, pairs):
-    """parts * 8 bytes per row (at most ceil(2048 / n) parts of >= 16 KiB), 8 + 4 per row, 8 per loss."""
+    """8 + 4 bytes per row, 8 per loss, and where rows are cut into parts (over 64 KiB) 8 for each of them: k
+    rows are cut into at most ceil(2048 / k) parts each, for any k <= n."""
     for code, es in ((0, 4), (1, 2), (2, 2)):
-        parts = max(1, min(-(-2048 // n), -(-m * es // 16384)))
+        parts = max(k * -(-2048 // k) for k in range(1, n + 1)) if m * es > 65536 else 0
         size = L.lib().kge_label_ws_size(n, m, code, pairs)
         least = n * 8 + n * 4 + max(n, pairs) * 8
-        assert least <= size <= least + n * parts * 8 + 4 * 256
+        assert least + parts * 8 <= size <= least + (n + 2048) * 8 + 4 * 256
