@@ -634,36 +634,22 @@ int kge_preference_loss(const void* s, int dtype, int64_t lds, int64_t n, int64_
  *   dA_t = sum_{i in t} u_i x_i^T,  dB_t = sum_{i in t} dy_i h_i^T        (zeros for an adapter without rows)
  * An id outside [-1, k) poisons its own row (NaN). */
 
-/* The rows in the order of their adapters: perm [n] (sorted position -> row), sid [n] (its adapter; k: none,
- * k + 1: out of range), start [k + 3] (first position of each group).  Stable, no atomics. */
-int kge_adapter_plan(const int64_t* ids, int64_t n, int64_t k, int32_t* perm, int32_t* sid, int32_t* start,
-                     void* stream);
+/* y [n, m].  save: kge_adapter_save_size bytes, 16-B aligned, of this call's own; for_backward 1: it holds the plan
+ * and h afterwards, as kge_adapter_backward takes them.  scales null: 1. */
+int64_t kge_adapter_save_size(int64_t n, int64_t d, int64_t k, int64_t r);
+int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
+                        int64_t m, const void* a, const void* b, int64_t k, int64_t r, const int64_t* ids,
+                        const float* scales, void* y, int64_t ldy, void* save, int64_t save_bytes, int for_backward,
+                        void* stream);
 
-/* out[i, 0 .. rp) = scales_t F_t v_perm[i] for the sorted rows i of an adapter (other rows undefined), v [n, cols].
- * F_t as [r, cols] (f_by_rank 1: A for h) or [cols, r] (f_by_rank 0: B for u); scales null: 1.
- * out: kge_adapter_shrink_rows(...) rows of rp floats, 16-B aligned, of which the first n are the result
- * (the others hold partial sums of the split columns). */
-int64_t kge_adapter_shrink_rows(int64_t n, int64_t cols, int64_t k, int64_t r);
-int kge_adapter_shrink(const void* v, int dtype, int64_t ldv, int64_t n, int64_t cols, const void* f, int f_by_rank,
-                       int64_t k, int64_t r, const float* scales, const int32_t* perm, const int32_t* start,
-                       float* out, int64_t out_rows, void* stream);
-
-/* y[perm[i], :] = W x_perm[i] + F_t h[i], F_t as [m, r] (f_by_rank 0: B) or [r, m] (f_by_rank 1: A, for dx from
- * dy, W transposed and u).  h [n, rp] as kge_adapter_shrink leaves it. */
-int kge_adapter_project(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
-                        int64_t m, const void* f, int f_by_rank, int64_t k, int64_t r, const float* h,
-                        const int32_t* perm, const int32_t* sid, void* y, int64_t ldy, void* stream);
-
-/* out_t = sum over the sorted rows i of adapter t of h[i, q] v[perm[i], c], as [cols, r] (out_by_rank 0: dB from dy
- * and h) or [r, cols] (out_by_rank 1: dA from x and u).  ws: kge_adapter_grads_ws_size floats (may be 0). */
-int64_t kge_adapter_grads_ws_size(int64_t n, int64_t cols, int64_t k, int64_t r, int dtype);
-int kge_adapter_grads(const void* v, int dtype, int64_t ldv, int64_t n, int64_t cols, const float* h, int64_t k,
-                      int64_t r, const int32_t* perm, const int32_t* start, void* out, int out_by_rank, float* ws,
-                      int64_t ws_elems, void* stream);
-
-/* dst [cols, rows] = src [rows, cols] transposed (KGE_DT_F32 / KGE_DT_BF16): W^T for dx */
-int kge_transpose(const void* src, int dtype, int64_t lds, int64_t rows, int64_t cols, void* dst, int64_t ldd,
-                  void* stream);
+/* dx [n, d], da [k, r, d], db [k, m, r] for dy [n, m]; each may be null.  ws: kge_adapter_backward_ws_size bytes
+ * (dx, da, db: whether that gradient is wanted), 16-B aligned, of this call's own. */
+int64_t kge_adapter_backward_ws_size(int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r, int dx, int da,
+                                     int db);
+int kge_adapter_backward(const void* dy, int dtype, int64_t lddy, int64_t n, int64_t m, const void* x, int64_t ldx,
+                         int64_t d, const void* w, int64_t ldw, const void* a, const void* b, int64_t k, int64_t r,
+                         const float* scales, void* save, int64_t save_bytes, void* dx, int64_t lddx, void* da,
+                         void* db, void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

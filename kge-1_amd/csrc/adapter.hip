@@ -53,11 +53,26 @@ struct Mma<float> {
   }
 };
 
-// `valid` (possibly <= 0) elements of a lane's 16 bytes, `stride` elements apart, the rest 0
-template <typename T, bool VEC>
-__device__ __forceinline__ u32x4 frag(const T* p, int64_t stride, int valid) {
+// `valid` (possibly <= 0) consecutive elements of a lane's 16 bytes, the rest 0.  Rows need no alignment beyond
+// their elements' own: the hardware splits a 16-byte load that crosses a line.
+template <typename T>
+__device__ __forceinline__ u32x4 frag(const T* p, int valid) {
   constexpr int N = Mma<T>::N;
-  if (VEC && valid >= N) return *reinterpret_cast<const u32x4*>(p);
+  if (valid >= N) {
+    u32x4 whole;
+    __builtin_memcpy(&whole, p, 16);
+    return whole;
+  }
+  typedef T vec __attribute__((ext_vector_type(N)));
+  vec v;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = e < valid ? p[e] : (T)0.f;
+  return __builtin_bit_cast(u32x4, v);
+}
+// the same, `stride` elements apart
+template <typename T>
+__device__ __forceinline__ u32x4 frag_strided(const T* p, int64_t stride, int valid) {
+  constexpr int N = Mma<T>::N;
   typedef T vec __attribute__((ext_vector_type(N)));
   vec v;
 #pragma unroll
@@ -67,22 +82,33 @@ __device__ __forceinline__ u32x4 frag(const T* p, int64_t stride, int valid) {
 
 // ---- plan: rows in the order of their adapters ----------------------------------------------------
 // Groups 0 .. k - 1: the adapters, k: rows without one (id -1), k + 1: ids out of range.  One workgroup
-// per group counts the ids below its own and lists its own in ascending row order: no atomics.
-constexpr int PT = 1024;
+// per group counts the ids below its own and lists its own in ascending row order: no atomics.  PU ids per
+// thread are in flight at once; a batch of up to PT PU rows is read once.
+constexpr int PT = 1024, PU = 8;
 
 __global__ void __launch_bounds__(PT) plan_kernel(const int64_t* __restrict__ ids, int n, int k,
                                                   int* __restrict__ perm, int* __restrict__ sid, int* __restrict__ start) {
-  __shared__ int red[2][PT / 64];
+  __shared__ int red[2][PT / 64], count[PU][PT / 64];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto group = [&](int i) {
-    const int64_t t = ids[i];
-    return t == -1 ? k : (t < 0 || t >= k ? k + 1 : (int)t);
+  int x[PU];
+  auto load = [&](int i0) {
+    int64_t v[PU];
+#pragma unroll
+    for (int u = 0; u < PU; ++u) v[u] = ids[min(i0 + u * PT + tid, n - 1)];
+#pragma unroll
+    for (int u = 0; u < PU; ++u) {
+      const int in = v[u] == -1 ? k : (v[u] < 0 || v[u] >= k ? k + 1 : (int)v[u]);
+      x[u] = i0 + u * PT + tid < n ? in : k + 2;
+    }
   };
   int less = 0, mine = 0;
-  for (int i = tid; i < n; i += PT) {
-    const int x = group(i);
-    less += x < g;
-    mine += x == g;
+  for (int i0 = 0; i0 < n; i0 += PT * PU) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < PU; ++u) {
+      less += x[u] < g;
+      mine += x[u] == g;
+    }
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
@@ -95,6 +121,7 @@ __global__ void __launch_bounds__(PT) plan_kernel(const int64_t* __restrict__ id
   }
   __syncthreads();
   less = mine = 0;
+#pragma unroll
   for (int w = 0; w < PT / 64; ++w) {
     less += red[0][w];
     mine += red[1][w];
@@ -105,24 +132,31 @@ __global__ void __launch_bounds__(PT) plan_kernel(const int64_t* __restrict__ id
   }
   if (mine == 0) return;  // the whole workgroup
   int at = less;
-  for (int i0 = 0; i0 < n; i0 += PT) {
-    __syncthreads();  // red of the previous round has been read
-    const int i = i0 + tid;
-    const bool is = i < n && group(i) == g;
-    const uint64_t mask = __ballot(is);
-    if (lane == 0) red[0][wave] = __popcll(mask);
+  for (int i0 = 0; i0 < n; i0 += PT * PU) {
+    if (n > PT * PU) load(i0);
+    __syncthreads();  // count of the previous round has been read
+    uint64_t mask[PU];
+#pragma unroll
+    for (int u = 0; u < PU; ++u) {
+      mask[u] = __ballot(x[u] == g);
+      if (lane == 0) count[u][wave] = __popcll(mask[u]);
+    }
     __syncthreads();
-    int before = 0, total = 0;
-    for (int w = 0; w < PT / 64; ++w) {
-      before += w < wave ? red[0][w] : 0;
-      total += red[0][w];
+#pragma unroll
+    for (int u = 0; u < PU; ++u) {
+      int before = 0, total = 0;
+#pragma unroll
+      for (int w = 0; w < PT / 64; ++w) {
+        before += w < wave ? count[u][w] : 0;
+        total += count[u][w];
+      }
+      if (x[u] == g) {
+        const int to = at + before + __popcll(mask[u] & ((1ull << lane) - 1));
+        perm[to] = i0 + u * PT + tid;
+        sid[to] = g;
+      }
+      at += total;
     }
-    if (is) {
-      const int to = at + before + __popcll(mask & ((1ull << lane) - 1));
-      perm[to] = i;
-      sid[to] = g;
-    }
-    at += total;
   }
 }
 
@@ -151,11 +185,11 @@ __device__ __forceinline__ Chunk chunk_of(int slot, const int* start, int k, int
 }
 
 // ---- shrink: out[i, 0 .. r) = scale_t F_t v_i for the sorted rows i --------------------------------
-// F_t element (rank q, column c) at f[t r cols + q fq + c fc].  grid: slots x rank blocks of 16 x splits
-// of the columns (each split a slab of its own).
-template <typename T, bool VV, bool FV>
+// F_t as [r, cols] (BY_RANK) or [cols, r].  grid: slots x rank blocks of 16 x splits of the columns (each
+// split a slab of its own).
+template <typename T, bool BY_RANK>
 __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, int64_t ldv, int n, int cols,
-                                                     const T* __restrict__ f, int64_t fq, int64_t fc, int k, int r, int rp,
+                                                     const T* __restrict__ f, int k, int r, int rp,
                                                      const float* __restrict__ scales, const int* __restrict__ perm,
                                                      const int* __restrict__ start, int per_split, float* __restrict__ out) {
   constexpr int N = Mma<T>::N, KC = Mma<T>::KC, UN = 4;
@@ -166,15 +200,16 @@ __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, in
   const int q = blockIdx.y * 16 + fr;
   const int c_lo = blockIdx.z * per_split, c_hi = min(cols, c_lo + per_split);
   const T* vr = v + (int64_t)perm[ch.row0 + min(fr, ch.rows - 1)] * ldv;
-  const T* fp = f + (int64_t)ch.t * r * cols + (int64_t)min(q, r - 1) * fq;
+  const int64_t fc = BY_RANK ? 1 : r;
+  const T* fp = f + (int64_t)ch.t * r * cols + (int64_t)min(q, r - 1) * (BY_RANK ? cols : 1);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int c0 = c_lo + wave * KC; c0 < c_hi; c0 += 4 * KC * UN) {
     u32x4 a[UN], b[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int c = c0 + u * 4 * KC + fs * N;
-      a[u] = frag<T, FV>(fp + (int64_t)c * fc, fc, c_hi - c);
-      b[u] = frag<T, VV>(vr + c, 1, c_hi - c);
+      a[u] = BY_RANK ? frag<T>(fp + c, c_hi - c) : frag_strided<T>(fp + (int64_t)c * fc, fc, c_hi - c);
+      b[u] = frag<T>(vr + c, c_hi - c);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) Mma<T>::run(acc, a[u], b[u]);
@@ -201,7 +236,10 @@ __global__ void __launch_bounds__(256) slabs_kernel(f32x4* __restrict__ x, int64
 }
 
 // ---- project: y[perm[i], :] = W x + F_t h_i -----------------------------------------------------------
-// F_t element (column c, rank q) at f[t r m + c fc + q fq].
+// F_t as [m, r] or (BY_RANK) [r, m].  128 x 128 tiles, four waves of 64 x 64, one 32-KiB LDS stage of 128
+// bytes of the summed axis; the next stage waits in registers.  One stage instead of two lets four workgroups
+// share a CU, whose phases (loads, products, adapters, stores) overlap: with the short summed axes of embedding
+// tables (512: 8 stages) a tile is latency, not MFMA time.
 constexpr int BM = 128, BN = 128, BKB = 128;  // rows of x, rows of W, bytes of the summed axis per stage
 
 // 16-byte slot of a 128-byte row, XOR-ed with the row: the 16 rows a fragment read touches then lie in
@@ -228,38 +266,81 @@ __device__ __forceinline__ u32x4 h_frag<__bf16>(const float* h, int q0, int fs) 
   }
   return __builtin_bit_cast(u32x4, o);
 }
-// the ranks of F that meet them
+
+// Adapter slices in LDS: 16 ranks of 128 columns, [column][16 ranks].
 template <typename T>
-__device__ __forceinline__ int f_rank(int q0, int fs) {
-  return sizeof(T) == 4 ? q0 + fs * 4 : q0 + (fs & 1) * 8;
+struct Slice {
+  static constexpr int ROW = 16 * sizeof(T), BYTES = BN * ROW, COUNT = (BM + BN) * BKB / BYTES;
+  // where a lane's part of column `col` starts: the ranks its h fragment holds
+  static __device__ __forceinline__ int at(int col, int fs) {
+    return col * ROW + (sizeof(T) == 4 ? fs : (fs & 1)) * 16;
+  }
+};
+__device__ __forceinline__ bool nonfinite(const u32x4& v, float) {
+  bool b = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b |= (v[e] & 0x7f800000u) == 0x7f800000u;
+  return b;
+}
+__device__ __forceinline__ bool nonfinite(const u32x4& v, __bf16) {
+  bool b = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b |= (v[e] & 0x7f800000u) == 0x7f800000u || (v[e] & 0x7f80u) == 0x7f80u;
+  return b;
 }
 
-template <typename T, bool XV, bool WV, bool FV>
-__global__ void __launch_bounds__(256) project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d,
-                                                      const T* __restrict__ w, int64_t ldw, int m,
-                                                      const T* __restrict__ f, int64_t fc, int64_t fq, int k, int r, int rp,
-                                                      const float* __restrict__ h, const int* __restrict__ perm,
-                                                      const int* __restrict__ sid, T* __restrict__ y, int64_t ldy,
-                                                      int row_tiles, int yvec) {
+// Copies ranks [q0, q0 + 16) of columns [m0, m0 + 128) of an adapter into its slice; whether anything in it is
+// infinite or NaN.
+template <typename T, bool BY_RANK>
+__device__ __forceinline__ bool stage_slice(const T* ft, int m, int r, int m0, int q0, unsigned char* to) {
+  constexpr int N = Mma<T>::N, P = 16 / N;  // 16-byte pieces per column
+  const int tid = threadIdx.x;
+  bool bad = false;
+#pragma unroll
+  for (int it = 0; it < BN * P / 256; ++it) {
+    const int piece = it * 256 + tid;
+    if (!BY_RANK) {
+      const int col = piece / P, q = q0 + piece % P * N, c = m0 + col;
+      const u32x4 v = c < m ? frag<T>(ft + (int64_t)c * r + q, r - q) : (u32x4){0u, 0u, 0u, 0u};
+      bad |= nonfinite(v, T());
+      *reinterpret_cast<u32x4*>(to + col * Slice<T>::ROW + piece % P * 16) = v;
+    } else {
+      typedef T vec __attribute__((ext_vector_type(N)));
+      const int q = piece / (BN / N), col = piece % (BN / N) * N, c = m0 + col;
+      const u32x4 v = q0 + q < r ? frag<T>(ft + (int64_t)(q0 + q) * m + c, m - c) : (u32x4){0u, 0u, 0u, 0u};
+      bad |= nonfinite(v, T());
+      const vec x = __builtin_bit_cast(vec, v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) *reinterpret_cast<T*>(to + (col + e) * Slice<T>::ROW + q * sizeof(T)) = x[e];
+    }
+  }
+  return bad;
+}
+
+template <typename T, bool BY_RANK>
+__global__ void __launch_bounds__(256, 3) project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d,
+                                                         const T* __restrict__ w, int64_t ldw, int m,
+                                                         const T* __restrict__ f, int k, int r, int rp,
+                                                         const float* __restrict__ h, const int* __restrict__ perm,
+                                                         const int* __restrict__ sid, T* __restrict__ y, int64_t ldy,
+                                                         int row_tiles, int yvec) {
   constexpr int N = Mma<T>::N, KE = BKB / sizeof(T), KC = Mma<T>::KC;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2][(BM + BN) * BKB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fs = lane >> 4;
-  const int wr = wave >> 1, wc = wave & 1;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[(BM + BN) * BKB];
+  __shared__ int owner[BM];
+  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fs = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1;
   const int tile = xcd_remap(blockIdx.x, gridDim.x);
   const int m0 = (tile / row_tiles) * BN, n0 = (tile % row_tiles) * BM;
 
   const T* src[8];
-  int kt[8];  // unused columns of the piece's row are found from its first column
+  const int kt = (tid & 7) * N;  // first column of this thread's pieces within a stage
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int row = (tid >> 3) + (j & 3) * 32;
-    if (j < 4) {
-      const int i = min(n0 + row, n - 1);
-      src[j] = x + (int64_t)perm[i] * ldx + (tid & 7) * N;
-    } else {
-      src[j] = w + (int64_t)min(m0 + row, m - 1) * ldw + (tid & 7) * N;
-    }
-    kt[j] = (tid & 7) * N;
+    if (j < 4)
+      src[j] = x + (int64_t)perm[min(n0 + row, n - 1)] * ldx + kt;
+    else
+      src[j] = w + (int64_t)min(m0 + row, m - 1) * ldw + kt;
   }
   f32x4 acc[4][4];
 #pragma unroll
@@ -268,68 +349,117 @@ __global__ void __launch_bounds__(256) project_kernel(const T* __restrict__ x, i
     for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
   u32x4 reg[8];
-  auto load = [&](int k0) {
+  auto load = [&](int k0) {  // a whole stage
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      reg[j] = j < 4 ? frag<T, XV>(src[j] + k0, 1, d - k0 - kt[j]) : frag<T, WV>(src[j] + k0, 1, d - k0 - kt[j]);
+    for (int j = 0; j < 8; ++j) __builtin_memcpy(&reg[j], src[j] + k0, 16);
   };
-  load(0);
-  int buf = 0;
+  if (KE <= d) load(0);
   for (int k0 = 0; k0 < d; k0 += KE) {
+    if (k0) __syncthreads();  // the previous stage has been read
+    if (k0 + KE <= d) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int row = (tid >> 3) + (j & 3) * 32 + (j < 4 ? 0 : BM);
-      *reinterpret_cast<u32x4*>(&lds[buf][lds_slot(row, tid & 7)]) = reg[j];
+      for (int j = 0; j < 8; ++j) {
+        const int row = (tid >> 3) + (j & 3) * 32 + (j < 4 ? 0 : BM);
+        *reinterpret_cast<u32x4*>(&lds[lds_slot(row, tid & 7)]) = reg[j];
+      }
+    } else {  // the rest of the summed axis, zeros behind it
+#pragma unroll 1
+      for (int row = tid >> 3; row < BM + BN; row += 32) {
+        const T* p = row < BM ? x + (int64_t)perm[min(n0 + row, n - 1)] * ldx : w + (int64_t)min(m0 + row - BM, m - 1) * ldw;
+        *reinterpret_cast<u32x4*>(&lds[lds_slot(row, tid & 7)]) = frag<T>(p + kt + k0, d - k0 - kt);
+      }
     }
     __syncthreads();
-    if (k0 + KE < d) load(k0 + KE);
+    if (k0 + 2 * KE <= d) load(k0 + KE);
 #pragma unroll
     for (int kc = 0; kc < KE / KC; ++kc) {
-      u32x4 xa[4], wb[4];
+      u32x4 wb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        wb[j] = *reinterpret_cast<const u32x4*>(&lds[lds_slot(BM + wc * 64 + j * 16 + fr, kc * 4 + fs)]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        xa[i] = *reinterpret_cast<const u32x4*>(&lds[buf][lds_slot(wr * 64 + i * 16 + fr, kc * 4 + fs)]);
-        wb[i] = *reinterpret_cast<const u32x4*>(&lds[buf][lds_slot(BM + wc * 64 + i * 16 + fr, kc * 4 + fs)]);
+        const u32x4 xa = *reinterpret_cast<const u32x4*>(&lds[lds_slot(wr * 64 + i * 16 + fr, kc * 4 + fs)]);
+        if constexpr (sizeof(T) == 4) {  // the four instructions on one accumulator four apart
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, wb[j])[e],
+                                                               __builtin_bit_cast(f32x4, xa)[e], acc[i][j], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) Mma<T>::run(acc[i][j], wb[j], xa);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) Mma<T>::run(acc[i][j], wb[j], xa[i]);
     }
-    buf ^= 1;
   }
 
-  // acc[i][j]: x row n0 + wr 64 + i 16 + fr, columns m0 + wc 64 + j 16 + 4 fs + reg
+  // acc[i][j]: x row n0 + wr 64 + i 16 + fr, columns m0 + wc 64 + j 16 + 4 fs + reg.
+  // The tile's adapters: sorted rows, so each is a run; slot = its number within the tile (-1: no adapter).
+  const int t_lo = n0 + lane < n ? sid[n0 + lane] : k, t_hi = n0 + 64 + lane < n ? sid[n0 + 64 + lane] : k;
+  const int p_lo = __shfl_up(t_lo, 1, 64), p_hi = __shfl_up(t_hi, 1, 64), mid = __shfl(t_lo, 63, 64);
+  const uint64_t b_lo = __ballot(t_lo < k && (lane == 0 || p_lo != t_lo));
+  const uint64_t b_hi = __ballot(t_hi < k && (lane == 0 ? mid : p_hi) != t_hi);
+  const uint64_t upto = lane == 63 ? ~0ull : (2ull << lane) - 1;
+  const int slot_lo = t_lo < k ? __popcll(b_lo & upto) - 1 : -1;
+  const int slot_hi = t_hi < k ? __popcll(b_lo) + __popcll(b_hi & upto) - 1 : -1;
+  const int slots = __popcll(b_lo) + __popcll(b_hi);
+  if (wave == 0) {
+    if ((b_lo >> lane) & 1) owner[slot_lo] = t_lo;
+    if ((b_hi >> lane) & 1) owner[slot_hi] = t_hi;
+  }
+  const int slot = wr ? slot_hi : slot_lo, t_own = wr ? t_hi : t_lo;  // of row wr 64 + lane
+
+  if (slots > 0) {
+    for (int q0 = 0; q0 < rp; q0 += 16) {
+      u32x4 hf[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        hf[i] = h_frag<T>(h + (int64_t)min(n0 + wr * 64 + i * 16 + fr, n - 1) * rp, q0, fs);
+      for (int s0 = 0; s0 < slots; s0 += Slice<T>::COUNT) {
+        const int count = min(Slice<T>::COUNT, slots - s0);
+        __syncthreads();  // the last stage or slices have been read, owner is written
+        bool bad = false;
+#pragma unroll 4
+        for (int s = 0; s < count; ++s)
+          bad |= stage_slice<T, BY_RANK>(f + (int64_t)owner[s0 + s] * r * m, m, r, m0, q0, lds + s * Slice<T>::BYTES);
+        const bool apart = __syncthreads_or(bad);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int si = __shfl(slot, i * 16 + fr, 64);
+          const int first = __builtin_amdgcn_readlane(slot, i * 16), end = __builtin_amdgcn_readlane(slot, i * 16 + 15);
+          if (first < 0) continue;  // no adapter from this row on
+          const int last = min(end < 0 ? slots - 1 : end, s0 + count - 1);
+          for (int s = max(first, s0); s <= last; ++s) {
+            const unsigned char* sl = lds + (s - s0) * Slice<T>::BYTES;
+            const bool own = si == s;
+            u32x4 hm;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hm[e] = own ? hf[i][e] : 0u;
+            if (!apart) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                Mma<T>::run(acc[i][j], *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
+            } else {  // an infinity times another row's 0 must not reach that row
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                f32x4 next = acc[i][j];  // the same sum in the same order for the adapter's own rows
+                Mma<T>::run(next, *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
+                if (own) acc[i][j] = next;
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = n0 + wr * 64 + i * 16 + fr;
-    const bool live = row < n;
-    const int t = live ? sid[row] : k;
-    const float* hr = h + (int64_t)min(row, n - 1) * rp;
-    unsigned todo = (unsigned)(__ballot(live && t < k) & 0xffffu);
-    while (todo) {  // one adapter after the other (uniform over the wave)
-      const int ta = __builtin_amdgcn_readlane(t, __builtin_ctz(todo));
-      todo &= ~(unsigned)(__ballot(t == ta) & 0xffffu);
-      const T* ft = f + (int64_t)ta * r * m;
-      f32x4 add[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) add[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      for (int q0 = 0; q0 < rp; q0 += 16) {
-        const u32x4 hb = t == ta ? h_frag<T>(hr, q0, fs) : (u32x4){0u, 0u, 0u, 0u};
-        const int q = f_rank<T>(q0, fs);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = min(m0 + wc * 64 + j * 16 + fr, m - 1);
-          Mma<T>::run(add[j], frag<T, FV>(ft + (int64_t)col * fc + (int64_t)q * fq, fq, r - q), hb);
-        }
-      }
-      if (t == ta) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += add[j];
-      }
-    }
-    if (!live) continue;
-    const float bad = t > k ? NAN : 0.f;  // an id out of range poisons its row
+    const float poison = __shfl(t_own, i * 16 + fr, 64) > k ? NAN : 0.f;  // an id out of range
+    if (row >= n) continue;
     T* yr = y + (int64_t)perm[row] * ldy;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -337,7 +467,7 @@ __global__ void __launch_bounds__(256) project_kernel(const T* __restrict__ x, i
       typedef T out4 __attribute__((ext_vector_type(4)));
       out4 o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (T)(acc[i][j][e] + bad);
+      for (int e = 0; e < 4; ++e) o[e] = (T)(acc[i][j][e] + poison);
       if (yvec && c + 4 <= m) {
         *reinterpret_cast<out4*>(yr + c) = o;
       } else {
@@ -349,11 +479,115 @@ __global__ void __launch_bounds__(256) project_kernel(const T* __restrict__ x, i
   }
 }
 
+// ---- few requests (serving): unsorted, no plan --------------------------------------------------------------
+// h_i of row i, ranks wave, wave + 4, .. by one wave each, to put(q, value)
+template <typename T, typename F>
+__device__ __forceinline__ void shrink_row(const T* __restrict__ xr, const T* __restrict__ at, int d, int r, float sc, int wave,
+                                           int lane, F put) {
+  constexpr int N = Mma<T>::N;
+  typedef T vec __attribute__((ext_vector_type(N)));
+  for (int q = wave; q < r; q += 4) {
+    float a = 0.f;
+    for (int c = lane * N; c < d; c += 64 * N) {
+      const vec u = __builtin_bit_cast(vec, frag<T>(xr + c, d - c));
+      const vec v = __builtin_bit_cast(vec, frag<T>(at + (int64_t)q * d + c, d - c));
+#pragma unroll
+      for (int e = 0; e < N; ++e) a = fmaf((float)u[e], (float)v[e], a);
+    }
+    a = wave_sum(a);
+    if (lane == 0) put(q, a * sc);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) shrink_few_kernel(const T* __restrict__ x, int64_t ldx, int d, const T* __restrict__ a,
+                                                         int k, int r, int rp, const int64_t* __restrict__ ids,
+                                                         const float* __restrict__ scales, float* __restrict__ h) {
+  const int row = blockIdx.x;
+  const int64_t t = ids[row];
+  if (t < 0 || t >= k) return;
+  float* hr = h + (int64_t)row * rp;
+  shrink_row<T>(x + row * ldx, a + t * r * d, d, r, scales ? scales[t] : 1.f, threadIdx.x >> 6, threadIdx.x & 63,
+                [&](int q, float v) { hr[q] = v; });
+}
+
+// A workgroup: 16 columns of y for up to 16 RB rows, its four waves a quarter of the summed axis each; then one
+// thread per value adds B_t h.  INLINE: h is worked out by every workgroup for itself (a row or two: A_t comes from
+// the L2, and a launch less).
+template <typename T, int RB, bool INLINE>
+__global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ x, int64_t ldx, int n, int d,
+                                                          const T* __restrict__ w, int64_t ldw, int m,
+                                                          const T* __restrict__ a, const T* __restrict__ b, int k, int r,
+                                                          int rp, const int64_t* __restrict__ ids,
+                                                          const float* __restrict__ scales, const float* __restrict__ h,
+                                                          T* __restrict__ y, int64_t ldy) {
+  constexpr int N = Mma<T>::N, KC = Mma<T>::KC, U = RB == 1 ? 4 : 2;
+  typedef T vec __attribute__((ext_vector_type(N)));
+  __shared__ f32x4 part[4][RB][64];
+  extern __shared__ float hs[];  // INLINE: [n][rp]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fs = lane >> 4;
+  const int m0 = blockIdx.x * 16;
+  const T* wp = w + (int64_t)min(m0 + fr, m - 1) * ldw + fs * N;
+  const T* xp[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) xp[rb] = x + (int64_t)min(rb * 16 + fr, n - 1) * ldx + fs * N;
+  f32x4 acc[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) acc[rb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int c0 = wave * KC; c0 < d; c0 += 4 * KC * U) {
+    u32x4 wf[U], xf[U][RB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 4 * KC;
+      wf[u] = frag<T>(wp + c, d - c - fs * N);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) xf[u][rb] = frag<T>(xp[rb] + c, d - c - fs * N);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) Mma<T>::run(acc[rb], wf[u], xf[u][rb]);
+  }
+  if (INLINE)
+    for (int i = 0; i < n; ++i) {
+      const int64_t t = ids[i];
+      if (t >= 0 && t < k)
+        shrink_row<T>(x + i * ldx, a + t * r * d, d, r, scales ? scales[t] : 1.f, wave, lane,
+                      [&](int q, float v) { hs[i * rp + q] = v; });
+    }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) part[wave][rb][lane] = acc[rb];
+  __syncthreads();
+  const int c = tid & 15, from = (c >> 2) * 16 + (tid >> 4), e = c & 3;  // part's lane of this thread's value
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = rb * 16 + (tid >> 4);
+    if (row >= n || m0 + c >= m) continue;
+    float v = (part[0][rb][from][e] + part[1][rb][from][e]) + (part[2][rb][from][e] + part[3][rb][from][e]);
+    const int64_t t = ids[row];
+    if (t >= 0 && t < k) {
+      const T* bt = b + (t * m + m0 + c) * r;
+      const float* hr = INLINE ? hs + row * rp : h + (int64_t)row * rp;
+      float add = 0.f;
+      for (int q = 0; q < r; q += N) {
+        const vec bv = __builtin_bit_cast(vec, frag<T>(bt + q, r - q));
+#pragma unroll
+        for (int z = 0; z < N; ++z)
+          if (q + z < r) add = fmaf((float)bv[z], hr[q + z], add);
+      }
+      v += add;
+    } else if (t != -1) {
+      v = NAN;  // an id out of range
+    }
+    y[(int64_t)row * ldy + m0 + c] = (T)v;
+  }
+}
+
 // ---- grads: out_t[q, c] = sum over the sorted rows i of adapter t of h[i, q] v[perm[i], c] -------------
 // One wave: 16 ranks x 16 N columns (a lane's 16 bytes of a row of v feed N instructions); the four
 // waves of a workgroup take every fourth group of four rows.  Adapters with more than `per` rows are cut into
 // chunks that write fp32 slabs, summed afterwards in ascending order.  An adapter without rows gets zeros.
-template <typename T, bool VV>
+template <typename T>
 __global__ void __launch_bounds__(256) grads_kernel(const T* __restrict__ v, int64_t ldv, int n, int cols,
                                                     const float* __restrict__ h, int rp, int k, int r,
                                                     const int* __restrict__ perm, const int* __restrict__ start, int per,
@@ -372,7 +606,7 @@ __global__ void __launch_bounds__(256) grads_kernel(const T* __restrict__ v, int
     const bool in = i + fs < ch.rows;
     const int row = ch.row0 + min(i + fs, ch.rows - 1);
     const float hv = in ? h[(int64_t)row * rp + q0 + fr] : 0.f;
-    const vec x = __builtin_bit_cast(vec, frag<T, VV>(v + (int64_t)perm[row] * ldv + c0, 1, in ? cols - c0 : 0));
+    const vec x = __builtin_bit_cast(vec, frag<T>(v + (int64_t)perm[row] * ldv + c0, in ? cols - c0 : 0));
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv, (float)x[j], acc[j], 0, 0, 0);
   }
@@ -434,161 +668,232 @@ __global__ void __launch_bounds__(256) transpose_kernel(const T* __restrict__ sr
 
 int elem_size(int dtype) { return dtype == KGE_DT_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == KGE_DT_F32 || dtype == KGE_DT_BF16; }
-bool vec_rows(const void* p, int64_t ld, int es) { return aligned16(p) && ld * es % 16 == 0; }
 bool ld_ok(int64_t ld, int64_t rows, int64_t cols) { return rows <= 1 || ld >= cols; }
-constexpr int64_t MAX_N = (int64_t)1 << 30;
+constexpr int64_t MAX_N = (int64_t)1 << 30, MAX_K = 1 << 20, MAX_R = 1024;
+constexpr int64_t FEW = 32;  // rows of the serving path
 int64_t rank_pad(int64_t r) { return (r + 15) / 16 * 16; }
+int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 template <typename F>
 int by_type(int dtype, F f) {
   return dtype == KGE_DT_F32 ? f((float*)nullptr) : f((__bf16*)nullptr);
 }
-template <typename F>
-int by_bool(bool b, F f) {
-  return b ? f(std::true_type{}) : f(std::false_type{});
+#define KGE_TRY(expr)      \
+  do {                     \
+    const int _r = (expr); \
+    if (_r) return _r;     \
+  } while (0)
+
+bool sizes_ok(int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r) {
+  return dtype_ok(dtype) && n >= 0 && n <= MAX_N && d >= 1 && d <= MAX_N && m >= 1 && m <= MAX_N && k >= 1 && k <= MAX_K &&
+         r >= 1 && r <= MAX_R;
 }
 
-// Splits of the summed columns of shrink: enough workgroups for two per CU where the rows' slots leave
-// CUs idle, at least 1024 columns each.
+// Splits of the summed columns of shrink: about four workgroups per CU where the rows' slots are fewer, at
+// least 512 columns each.
 int shrink_splits(int64_t n, int64_t cols, int64_t k, int64_t rp) {
   const int64_t groups = (std::min<int64_t>(n / 16 + k, n) + 1) * (rp / 16);
-  const int64_t want = (2 * kge_num_cus() + groups - 1) / groups, most = std::max<int64_t>(1, cols / 1024);
+  const int64_t want = (4 * kge_num_cus() + groups - 1) / groups, most = std::max<int64_t>(1, cols / 512);
   return (int)std::max<int64_t>(1, std::min(want, most));
 }
 
-// Rows of one chunk of grads: a multiple of 64, so that the launch has about 2048 workgroups
-int64_t grads_per(int64_t n, int64_t cols, int64_t k, int64_t r, int es) {
+// Rows of one chunk of grads: at least 256 (16 rounds of a workgroup), so that few adapters need their
+// chunks joined; more where the launch would exceed about 2048 workgroups
+int64_t grads_per(int64_t n, int64_t cols, int64_t r, int es) {
   const int64_t blocks = ((cols * es + 255) / 256) * (rank_pad(r) / 16);
   const int64_t chunks = std::max<int64_t>(1, 2048 / blocks);
-  return std::max<int64_t>(64, ((n + chunks - 1) / chunks + 63) / 64 * 64);
+  return std::max<int64_t>(256, ((n + chunks - 1) / chunks + 63) / 64 * 64);
+}
+int64_t grads_ws(int64_t n, int64_t cols, int64_t k, int64_t r, int es) {
+  const int64_t per = grads_per(n, cols, r, es);
+  return n <= per ? 0 : (n / per + k) * r * cols * 4;
+}
+
+// what the forward pass leaves for the backward one: the plan and h
+struct Save {
+  int *perm, *sid, *start;
+  float* h;
+  int64_t bytes;
+};
+Save save_of(void* base, int64_t n, int64_t d, int64_t k, int64_t r) {
+  char* b = (char*)base;
+  Save s;
+  int64_t o = 0;
+  s.perm = (int*)(b + o);
+  o += round256(n * 4);
+  s.sid = (int*)(b + o);
+  o += round256(n * 4);
+  s.start = (int*)(b + o);
+  o += round256((k + 3) * 4);
+  s.h = (float*)(b + o);
+  o += round256(n * rank_pad(r) * shrink_splits(n, d, k, rank_pad(r)) * 4);
+  s.bytes = o;
+  return s;
+}
+
+struct BackWs {
+  float* u;
+  void* wt;
+  int64_t ldwt;
+  float* slabs;
+  int64_t bytes;
+};
+BackWs back_ws_of(void* base, int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r, bool dx, bool da, bool db) {
+  const int es = elem_size(dtype);
+  char* b = (char*)base;
+  BackWs s;
+  int64_t o = 0;
+  s.u = (float*)(b + o);
+  if (dx || da) o += round256(n * rank_pad(r) * shrink_splits(n, m, k, rank_pad(r)) * 4);
+  s.ldwt = (m * es + 15) / 16 * 16 / es;
+  s.wt = b + o;
+  if (dx) o += round256(d * s.ldwt * es);
+  s.slabs = (float*)(b + o);
+  o += round256(std::max(da ? grads_ws(n, d, k, r, es) : 0, db ? grads_ws(n, m, k, r, es) : 0));
+  s.bytes = o;
+  return s;
+}
+
+int run_plan(const int64_t* ids, int64_t n, int64_t k, const Save& s, hipStream_t st) {
+  plan_kernel<<<dim3((unsigned)(k + 2)), dim3(PT), 0, st>>>(ids, (int)n, (int)k, s.perm, s.sid, s.start);
+  KGE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, bool BY_RANK>
+int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int64_t k, int64_t r, const float* scales,
+               const Save& s, float* out, hipStream_t st) {
+  const int rp = (int)rank_pad(r), splits = shrink_splits(n, cols, k, rp);
+  const int64_t per_split = ((cols + splits - 1) / splits + 127) / 128 * 128;
+  shrink_kernel<T, BY_RANK><<<dim3((unsigned)(n / 16 + k), (unsigned)(rp / 16), (unsigned)splits), dim3(256), 0, st>>>(
+      v, ldv, (int)n, (int)cols, f, (int)k, (int)r, rp, scales, s.perm, s.start, (int)per_split, out);
+  KGE_CHECK_LAUNCH();
+  if (splits == 1) return 0;
+  const int64_t count = n * rp / 4;
+  slabs_kernel<<<dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st>>>((f32x4*)out, count, splits);
+  KGE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, bool BY_RANK>
+int run_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
+                int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
+  const int64_t row_tiles = (n + BM - 1) / BM, tiles = row_tiles * ((m + BN - 1) / BN);
+  KGE_REQUIRE(tiles < ((int64_t)1 << 31));
+  const int yvec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T))) == 0 && ldy % 4 == 0;
+  project_kernel<T, BY_RANK><<<dim3((unsigned)tiles), dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k,
+                                                                          (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy,
+                                                                          (int)row_tiles, yvec);
+  KGE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+int run_grads(const T* v, int64_t ldv, int64_t n, int64_t cols, const float* h, int64_t k, int64_t r, const Save& s, T* out,
+              bool by_rank, float* slabs, hipStream_t st) {
+  const int64_t per = grads_per(n, cols, r, sizeof(T)), blocks = (cols * sizeof(T) + 255) / 256;
+  const int64_t oc = by_rank ? 1 : r, oq = by_rank ? cols : 1;
+  KGE_REQUIRE(blocks <= 65535);
+  grads_kernel<T><<<dim3((unsigned)(n / per + k), (unsigned)blocks, (unsigned)(rank_pad(r) / 16)), dim3(256), 0, st>>>(
+      v, ldv, (int)n, (int)cols, h, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per, out, oc, oq, slabs);
+  KGE_CHECK_LAUNCH();
+  if (n <= per) return 0;
+  const int64_t join = std::max<int64_t>(1, std::min<int64_t>((r * cols + 255) / 256, 64));
+  grads_join_kernel<T><<<dim3((unsigned)k, (unsigned)join), dim3(256), 0, st>>>(slabs, s.start, (int)per, (int)cols, (int)r,
+                                                                                out, oc, oq);
+  KGE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int RB>
+int run_few(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* a, const T* b,
+            int64_t k, int64_t r, const int64_t* ids, const float* scales, float* h, T* y, int64_t ldy, hipStream_t st) {
+  const int rp = (int)rank_pad(r);
+  const dim3 grid((unsigned)((m + 15) / 16));
+  if (RB == 1 && n * r * d * (int64_t)sizeof(T) <= 32768 && n * rp * 4 <= 16384) {
+    project_few_kernel<T, 1, true><<<grid, dim3(256), (size_t)(n * rp * 4), st>>>(
+        x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r, rp, ids, scales, nullptr, y, ldy);
+    KGE_CHECK_LAUNCH();
+    return 0;
+  }
+  shrink_few_kernel<T><<<dim3((unsigned)n), dim3(256), 0, st>>>(x, ldx, (int)d, a, (int)k, (int)r, rp, ids, scales, h);
+  KGE_CHECK_LAUNCH();
+  project_few_kernel<T, RB, false><<<grid, dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r,
+                                                               rp, ids, scales, h, y, ldy);
+  KGE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+int run_transpose(const T* src, int64_t lds, int64_t rows, int64_t cols, T* dst, int64_t ldd, hipStream_t st) {
+  // the y dimension of a grid is limited: bands of rows
+  for (int64_t r0 = 0; r0 < rows; r0 += 65535 * (int64_t)32) {
+    const int64_t nr = std::min<int64_t>(rows - r0, 65535 * (int64_t)32);
+    transpose_kernel<T><<<dim3((unsigned)((cols + 31) / 32), (unsigned)((nr + 31) / 32)), dim3(256), 0, st>>>(
+        src + r0 * lds, lds, (int)nr, (int)cols, dst + r0, ldd);
+    KGE_CHECK_LAUNCH();
+  }
+  return 0;
 }
 
 }  // namespace
 
-extern "C" int kge_adapter_plan(const int64_t* ids, int64_t n, int64_t k, int32_t* perm, int32_t* sid, int32_t* start,
-                                void* stream) {
-  KGE_REQUIRE(n >= 0 && n <= MAX_N && k >= 1 && k <= (1 << 20) && start && (n == 0 || (ids && perm && sid)));
-  plan_kernel<<<dim3((unsigned)(k + 2)), dim3(PT), 0, as_stream(stream)>>>(ids, (int)n, (int)k, perm, sid, start);
-  KGE_CHECK_LAUNCH();
-  return 0;
+extern "C" int64_t kge_adapter_save_size(int64_t n, int64_t d, int64_t k, int64_t r) {
+  return sizes_ok(KGE_DT_F32, n, d, 1, k, r) ? save_of(nullptr, n, d, k, r).bytes : 0;
 }
 
-extern "C" int64_t kge_adapter_shrink_rows(int64_t n, int64_t cols, int64_t k, int64_t r) {
-  if (n < 0 || cols < 1 || k < 1 || r < 1) return 0;
-  return n * shrink_splits(n, cols, k, rank_pad(r));
-}
-
-extern "C" int kge_adapter_shrink(const void* v, int dtype, int64_t ldv, int64_t n, int64_t cols, const void* f,
-                                  int f_by_rank, int64_t k, int64_t r, const float* scales, const int32_t* perm,
-                                  const int32_t* start, float* out, int64_t out_rows, void* stream) {
-  KGE_REQUIRE(dtype_ok(dtype) && n >= 0 && n <= MAX_N && cols >= 1 && cols <= MAX_N && k >= 1 && k <= (1 << 20) && r >= 1 &&
-              r <= 1024 && ld_ok(ldv, n, cols));
-  if (n == 0) return 0;
-  const int es = elem_size(dtype), rp = (int)rank_pad(r);
-  const int splits = shrink_splits(n, cols, k, rp);
-  KGE_REQUIRE(v && f && perm && start && out && aligned16(out) && out_rows >= n * splits);
-  const int64_t per_split = ((cols + splits - 1) / splits + 127) / 128 * 128;
-  const int64_t fq = f_by_rank ? cols : 1, fc = f_by_rank ? 1 : r;
-  const dim3 grid((unsigned)(n / 16 + k), (unsigned)(rp / 16), (unsigned)splits);
-  int rc = by_type(dtype, [&](auto* tag) {
-    typedef typename std::remove_pointer<decltype(tag)>::type T;
-    return by_bool(vec_rows(v, ldv, es), [&](auto vv) {
-      return by_bool(f_by_rank && vec_rows(f, cols, es), [&](auto fv) -> int {
-        shrink_kernel<T, vv.value, fv.value><<<grid, dim3(256), 0, as_stream(stream)>>>(
-            (const T*)v, ldv, (int)n, (int)cols, (const T*)f, fq, fc, (int)k, (int)r, rp, scales, perm, start,
-            (int)per_split, out);
-        KGE_CHECK_LAUNCH();
-        return 0;
-      });
-    });
-  });
-  if (rc || splits == 1) return rc;
-  const int64_t count = n * rp / 4;
-  slabs_kernel<<<dim3((unsigned)((count + 255) / 256)), dim3(256), 0, as_stream(stream)>>>((f32x4*)out, count, splits);
-  KGE_CHECK_LAUNCH();
-  return 0;
-}
-
-extern "C" int kge_adapter_project(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
-                                   int64_t m, const void* f, int f_by_rank, int64_t k, int64_t r, const float* h,
-                                   const int32_t* perm, const int32_t* sid, void* y, int64_t ldy, void* stream) {
-  KGE_REQUIRE(dtype_ok(dtype) && n >= 0 && n <= MAX_N && d >= 1 && d <= MAX_N && m >= 1 && m <= MAX_N && k >= 1 &&
-              k <= (1 << 20) && r >= 1 && r <= 1024 && ld_ok(ldx, n, d) && ld_ok(ldw, m, d) && ld_ok(ldy, n, m));
-  if (n == 0) return 0;
-  const int es = elem_size(dtype), rp = (int)rank_pad(r);
-  KGE_REQUIRE(x && w && f && h && perm && sid && y && aligned16(h));
-  const int64_t fc = f_by_rank ? 1 : r, fq = f_by_rank ? m : 1;
-  const int64_t row_tiles = (n + BM - 1) / BM, tiles = row_tiles * ((m + BN - 1) / BN);
-  KGE_REQUIRE(tiles < ((int64_t)1 << 31));
-  const int yvec = (reinterpret_cast<uintptr_t>(y) % (4 * es)) == 0 && ldy % 4 == 0;
-  return by_type(dtype, [&](auto* tag) {
-    typedef typename std::remove_pointer<decltype(tag)>::type T;
-    return by_bool(vec_rows(x, ldx, es), [&](auto xv) {
-      return by_bool(vec_rows(w, ldw, es), [&](auto wv) {
-        return by_bool(!f_by_rank && vec_rows(f, r, es), [&](auto fv) -> int {
-          project_kernel<T, xv.value, wv.value, fv.value><<<dim3((unsigned)tiles), dim3(256), 0, as_stream(stream)>>>(
-              (const T*)x, ldx, (int)n, (int)d, (const T*)w, ldw, (int)m, (const T*)f, fc, fq, (int)k, (int)r, rp, h, perm,
-              sid, (T*)y, ldy, (int)row_tiles, yvec);
-          KGE_CHECK_LAUNCH();
-          return 0;
-        });
-      });
-    });
-  });
-}
-
-extern "C" int64_t kge_adapter_grads_ws_size(int64_t n, int64_t cols, int64_t k, int64_t r, int dtype) {
-  if (n < 0 || cols < 1 || k < 1 || r < 1 || !dtype_ok(dtype)) return 0;
-  const int64_t per = grads_per(n, cols, k, r, elem_size(dtype));
-  return n <= per ? 0 : (n / per + k) * r * cols;
-}
-
-extern "C" int kge_adapter_grads(const void* v, int dtype, int64_t ldv, int64_t n, int64_t cols, const float* h, int64_t k,
-                                 int64_t r, const int32_t* perm, const int32_t* start, void* out, int out_by_rank, float* ws,
-                                 int64_t ws_elems, void* stream) {
-  KGE_REQUIRE(dtype_ok(dtype) && n >= 0 && n <= MAX_N && cols >= 1 && cols <= MAX_N && k >= 1 && k <= (1 << 20) && r >= 1 &&
-              r <= 1024 && ld_ok(ldv, n, cols) && start && out && (n == 0 || (v && h && perm)));
-  const int es = elem_size(dtype), rp = (int)rank_pad(r);
-  const int64_t per = grads_per(n, cols, k, r, es);
-  const bool join = n > per;
-  KGE_REQUIRE(!join || (ws && ws_elems >= (n / per + k) * r * cols));
-  const int64_t oc = out_by_rank ? 1 : r, oq = out_by_rank ? cols : 1;
-  const int64_t col_blocks = (cols * es + 255) / 256;
-  KGE_REQUIRE(col_blocks <= 65535);
-  return by_type(dtype, [&](auto* tag) {
-    typedef typename std::remove_pointer<decltype(tag)>::type T;
-    int rc = by_bool(n > 0 && vec_rows(v, ldv, es), [&](auto vv) -> int {
-      grads_kernel<T, vv.value><<<dim3((unsigned)(n / per + k), (unsigned)col_blocks, (unsigned)(rp / 16)), dim3(256), 0,
-                                  as_stream(stream)>>>((const T*)v, ldv, (int)n, (int)cols, h, rp, (int)k, (int)r, perm,
-                                                       start, (int)per, (T*)out, oc, oq, ws);
-      KGE_CHECK_LAUNCH();
-      return 0;
-    });
-    if (rc || !join) return rc;
-    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((r * cols + 1023) / 1024, 64));
-    grads_join_kernel<T><<<dim3((unsigned)k, (unsigned)blocks), dim3(256), 0, as_stream(stream)>>>(
-        ws, start, (int)per, (int)cols, (int)r, (T*)out, oc, oq);
-    KGE_CHECK_LAUNCH();
-    return 0;
-  });
-}
-
-extern "C" int kge_transpose(const void* src, int dtype, int64_t lds, int64_t rows, int64_t cols, void* dst, int64_t ldd,
-                             void* stream) {
-  KGE_REQUIRE(dtype_ok(dtype) && rows >= 0 && cols >= 0 && rows <= MAX_N && cols <= MAX_N && ld_ok(lds, rows, cols) &&
-              ld_ok(ldd, cols, rows));
-  if (rows == 0 || cols == 0) return 0;
-  const int64_t bx = (cols + 31) / 32, by = (rows + 31) / 32;
-  KGE_REQUIRE(src && dst && by <= 65535 * (int64_t)1024);
+extern "C" int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
+                                   int64_t m, const void* a, const void* b, int64_t k, int64_t r, const int64_t* ids,
+                                   const float* scales, void* y, int64_t ldy, void* save, int64_t save_bytes, int for_backward,
+                                   void* stream) {
+  KGE_REQUIRE(sizes_ok(dtype, n, d, m, k, r) && ld_ok(ldx, n, d) && ld_ok(ldw, m, d) && ld_ok(ldy, n, m));
+  KGE_REQUIRE(save && aligned16(save) && save_bytes >= save_of(save, n, d, k, r).bytes);
+  KGE_REQUIRE(n == 0 || (x && w && a && b && ids && y));
+  const Save s = save_of(save, n, d, k, r);
+  const hipStream_t st = as_stream(stream);
   return by_type(dtype, [&](auto* tag) -> int {
     typedef typename std::remove_pointer<decltype(tag)>::type T;
-    // the y dimension of a grid is limited: bands of rows
-    for (int64_t b = 0; b < by; b += 65535) {
-      const int64_t r0 = b * 32, nr = std::min<int64_t>(rows - r0, 65535 * (int64_t)32);
-      transpose_kernel<T><<<dim3((unsigned)bx, (unsigned)((nr + 31) / 32)), dim3(256), 0, as_stream(stream)>>>(
-          (const T*)src + r0 * lds, lds, (int)nr, (int)cols, (T*)dst + r0, ldd);
-      KGE_CHECK_LAUNCH();
+    const T *xt = (const T*)x, *wt = (const T*)w, *at = (const T*)a, *bt = (const T*)b;
+    T* yt = (T*)y;
+    if (!for_backward && n <= FEW) {
+      if (n == 0) return 0;
+      return n <= 16 ? run_few<T, 1>(xt, ldx, n, d, wt, ldw, m, at, bt, k, r, ids, scales, s.h, yt, ldy, st)
+                     : run_few<T, 2>(xt, ldx, n, d, wt, ldw, m, at, bt, k, r, ids, scales, s.h, yt, ldy, st);
     }
+    KGE_TRY(run_plan(ids, n, k, s, st));
+    if (n == 0) return 0;
+    KGE_TRY((run_shrink<T, true>(xt, ldx, n, d, at, k, r, scales, s, s.h, st)));
+    return run_project<T, false>(xt, ldx, n, d, wt, ldw, m, bt, k, r, s.h, s, yt, ldy, st);
+  });
+}
+
+extern "C" int64_t kge_adapter_backward_ws_size(int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r, int dx,
+                                                int da, int db) {
+  return sizes_ok(dtype, n, d, m, k, r) ? back_ws_of(nullptr, dtype, n, d, m, k, r, dx, da, db).bytes : 0;
+}
+
+extern "C" int kge_adapter_backward(const void* dy, int dtype, int64_t lddy, int64_t n, int64_t m, const void* x, int64_t ldx,
+                                    int64_t d, const void* w, int64_t ldw, const void* a, const void* b, int64_t k, int64_t r,
+                                    const float* scales, void* save, int64_t save_bytes, void* dx, int64_t lddx, void* da,
+                                    void* db, void* ws, int64_t ws_bytes, void* stream) {
+  KGE_REQUIRE(sizes_ok(dtype, n, d, m, k, r) && ld_ok(lddy, n, m) && ld_ok(ldx, n, d) && ld_ok(ldw, m, d) &&
+              ld_ok(lddx, n, d));
+  KGE_REQUIRE(save && aligned16(save) && save_bytes >= save_of(save, n, d, k, r).bytes);
+  KGE_REQUIRE(n == 0 || (dy && x && w && a && b));
+  const Save s = save_of(save, n, d, k, r);
+  const BackWs q = back_ws_of(ws, dtype, n, d, m, k, r, dx, da, db);
+  KGE_REQUIRE(ws_bytes >= q.bytes && (q.bytes == 0 || (ws && aligned16(ws))));
+  const hipStream_t st = as_stream(stream);
+  return by_type(dtype, [&](auto* tag) -> int {
+    typedef typename std::remove_pointer<decltype(tag)>::type T;
+    const T *dyt = (const T*)dy, *xt = (const T*)x, *wt = (const T*)w, *at = (const T*)a, *bt = (const T*)b;
+    if (n > 0 && (dx || da)) KGE_TRY((run_shrink<T, false>(dyt, lddy, n, m, bt, k, r, scales, s, q.u, st)));
+    if (n > 0 && dx) {
+      KGE_TRY(run_transpose<T>(wt, ldw, m, d, (T*)q.wt, q.ldwt, st));
+      KGE_TRY((run_project<T, true>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, at, k, r, q.u, s, (T*)dx, lddx, st)));
+    }
+    if (da) KGE_TRY(run_grads<T>(xt, ldx, n, d, q.u, k, r, s, (T*)da, true, q.slabs, st));
+    if (db) KGE_TRY(run_grads<T>(dyt, lddy, n, m, s.h, k, r, s, (T*)db, false, q.slabs, st));
     return 0;
   });
 }

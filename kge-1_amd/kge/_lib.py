@@ -118,14 +118,12 @@ SIGNATURES = {
                          _P, _I64, _P], _I),
     "kge_preference_loss": ([_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _D, _D, _I, _D, _D, _P, _P, _P, _P, _P, _P,
                              _I64, _P, _I64, _P], _I),
-    "kge_adapter_plan": ([_P, _I64, _I64, _P, _P, _P, _P], _I),
-    "kge_adapter_shrink_rows": ([_I64, _I64, _I64, _I64], _I64),
-    "kge_adapter_shrink": ([_P, _I, _I64, _I64, _I64, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _P], _I),
-    "kge_adapter_project": ([_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _P],
-                            _I),
-    "kge_adapter_grads_ws_size": ([_I64, _I64, _I64, _I64, _I], _I64),
-    "kge_adapter_grads": ([_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I, _P, _I64, _P], _I),
-    "kge_transpose": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "kge_adapter_save_size": ([_I64, _I64, _I64, _I64], _I64),
+    "kge_adapter_forward": ([_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I,
+                             _P], _I),
+    "kge_adapter_backward_ws_size": ([_I, _I64, _I64, _I64, _I64, _I64, _I, _I, _I], _I64),
+    "kge_adapter_backward": ([_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P,
+                              _I64, _P, _P, _P, _I64, _P], _I),
     "kge_bce_grad_planes": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _F, _F, _P, _I64, _P, _P], _I),
 }
 

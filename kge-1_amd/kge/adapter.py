@@ -21,7 +21,7 @@ from .label_losses import _capturing, on_device_of
 MAX_RANK = 1024
 
 
-def _matrix(t: torch.Tensor, what: str) -> torch.Tensor:
+def _matrix(t: torch.Tensor) -> torch.Tensor:
     """[rows, cols] with unit column stride and rows that do not overlap."""
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
@@ -40,89 +40,43 @@ def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     return buf if ld == cols else buf[:, :cols]
 
 
-class _Plan:
-    """The rows of a batch in the order of their adapters."""
-
-    def __init__(self, ids: torch.Tensor, k: int):
-        n = ids.numel()
-        buf = torch.empty(2 * n + k + 3, device=ids.device, dtype=torch.int32)
-        self.perm, self.sid, self.start = buf[:n], buf[n:2 * n], buf[2 * n:]
-        L._check(L.lib().kge_adapter_plan(L.ptr(ids), n, k, L.ptr(self.perm), L.ptr(self.sid), L.ptr(self.start),
-                                          L.stream()), "kge_adapter_plan")
-
-    @staticmethod
-    def of(tensors):
-        plan = object.__new__(_Plan)
-        plan.perm, plan.sid, plan.start = tensors
-        return plan
-
-
-def _shrink(v, f, by_rank, k, r, scales, plan):
-    n, cols = v.shape
-    rows = L.lib().kge_adapter_shrink_rows(n, cols, k, r)
-    out = torch.empty(rows, (r + 15) // 16 * 16, device=v.device, dtype=torch.float32)
-    L._check(L.lib().kge_adapter_shrink(L.ptr(v), L.DTYPES[v.dtype], _ld(v), n, cols, L.ptr(f), int(by_rank), k, r,
-                                        L.ptr(scales), L.ptr(plan.perm), L.ptr(plan.start), L.ptr(out), rows,
-                                        L.stream()), "kge_adapter_shrink")
-    return out
-
-
-def _project(x, w, f, by_rank, k, r, h, plan):
+def _forward(x, w, a, b, ids, scales, for_backward):
+    """(y, what the backward pass needs)"""
     n, d = x.shape
-    m = w.shape[0]
+    m, (k, r) = w.shape[0], a.shape[:2]
     y = _padded(n, m, x)
-    L._check(L.lib().kge_adapter_project(L.ptr(x), L.DTYPES[x.dtype], _ld(x), n, d, L.ptr(w), _ld(w), m, L.ptr(f),
-                                         int(by_rank), k, r, L.ptr(h), L.ptr(plan.perm), L.ptr(plan.sid), L.ptr(y),
-                                         _ld(y), L.stream()), "kge_adapter_project")
-    return y
-
-
-def _grads(v, h, k, r, plan, by_rank):
-    n, cols = v.shape
-    out = torch.empty((k, r, cols) if by_rank else (k, cols, r), device=v.device, dtype=v.dtype)
-    size = L.lib().kge_adapter_grads_ws_size(n, cols, k, r, L.DTYPES[v.dtype])
-    ws = torch.empty(size, device=v.device, dtype=torch.float32) if size > 0 else None
-    L._check(L.lib().kge_adapter_grads(L.ptr(v), L.DTYPES[v.dtype], _ld(v), n, cols, L.ptr(h), k, r, L.ptr(plan.perm),
-                                       L.ptr(plan.start), L.ptr(out), int(by_rank), L.ptr(ws), size, L.stream()),
-             "kge_adapter_grads")
-    return out
-
-
-def _transposed(w):
-    out = _padded(w.shape[1], w.shape[0], w)
-    L._check(L.lib().kge_transpose(L.ptr(w), L.DTYPES[w.dtype], _ld(w), w.shape[0], w.shape[1], L.ptr(out), _ld(out),
-                                   L.stream()), "kge_transpose")
-    return out
+    size = L.lib().kge_adapter_save_size(n, d, k, r)
+    save = torch.empty(size, device=x.device, dtype=torch.uint8)
+    L._check(L.lib().kge_adapter_forward(L.ptr(x), L.DTYPES[x.dtype], _ld(x), n, d, L.ptr(w), _ld(w), m, L.ptr(a), L.ptr(b),
+                                         k, r, L.ptr(ids), L.ptr(scales), L.ptr(y), _ld(y), L.ptr(save), size,
+                                         int(for_backward), L.stream()), "kge_adapter_forward")
+    return y, save
 
 
 class _AdaptedProjection(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, a, b, ids, scales):
-        k, r = a.shape[0], a.shape[1]
-        plan = _Plan(ids, k)
-        h = _shrink(x, a, True, k, r, scales, plan)
-        y = _project(x, w, b, False, k, r, h, plan)
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(x, w, a, b, scales, h, plan.perm, plan.sid, plan.start)
+        y, save = _forward(x, w, a, b, ids, scales, True)
+        ctx.save_for_backward(x, w, a, b, scales, save)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, a, b, scales, h, *plan = ctx.saved_tensors
-        plan = _Plan.of(plan)
-        k, r = a.shape[0], a.shape[1]
-        dx = da = db = None
+        x, w, a, b, scales, save = ctx.saved_tensors
+        n, d = x.shape
+        m, (k, r) = w.shape[0], a.shape[:2]
+        want = [ctx.needs_input_grad[i] for i in (0, 2, 3)]
         with on_device_of(x):
-            dy = _matrix(dy, "dy")
-            if ctx.needs_input_grad[0] or ctx.needs_input_grad[2]:
-                u = _shrink(dy, b, False, k, r, scales, plan)
-            if ctx.needs_input_grad[0]:
-                dx = _project(dy, _transposed(w), a, True, k, r, u, plan)
-            if ctx.needs_input_grad[2]:
-                da = _grads(x, u, k, r, plan, True)
-            if ctx.needs_input_grad[3]:
-                db = _grads(dy, h, k, r, plan, False)
+            dy = _matrix(dy)
+            dx = _padded(n, d, x) if want[0] else None
+            da, db = (torch.empty_like(t) if w_ else None for t, w_ in zip((a, b), want[1:]))
+            size = L.lib().kge_adapter_backward_ws_size(L.DTYPES[x.dtype], n, d, m, k, r, *want)
+            ws = torch.empty(size, device=x.device, dtype=torch.uint8)
+            L._check(L.lib().kge_adapter_backward(
+                L.ptr(dy), L.DTYPES[dy.dtype], _ld(dy), n, m, L.ptr(x), _ld(x), d, L.ptr(w), _ld(w), L.ptr(a), L.ptr(b), k, r,
+                L.ptr(scales), L.ptr(save), save.numel(), L.ptr(dx), _ld(dx) if want[0] else d, L.ptr(da), L.ptr(db),
+                L.ptr(ws), size, L.stream()), "kge_adapter_backward")
         return dx, None, da, db, None, None
 
 
@@ -135,10 +89,11 @@ def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: tor
     or bf16 (scales in any floating type, used in fp32).  Differentiable in x, a and b."""
     if x.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"x: expected float32 or bfloat16, got {x.dtype}")
+    dtype, dev = x.dtype, x.get_device()  # (-1: CPU)
     for t, dim, what in ((x, 2, "x [n, d]"), (w, 2, "w [m, d]"), (a, 3, "a [k, r, d]"), (b, 3, "b [k, m, r]")):
-        if t.dim() != dim or t.dtype != x.dtype:
-            raise ValueError(f"{what}: expected {dim} dimensions of {x.dtype}, got {list(t.shape)} {t.dtype}")
-        if t.device != x.device:
+        if t.dim() != dim or t.dtype != dtype:
+            raise ValueError(f"{what}: expected {dim} dimensions of {dtype}, got {list(t.shape)} {t.dtype}")
+        if t.get_device() != dev:
             raise ValueError(f"{what}: on {t.device}, x is on {x.device}")
     (n, d), m, (k, r) = x.shape, w.shape[0], a.shape[:2]
     if w.shape[1] != d or a.shape[2] != d or tuple(b.shape) != (k, m, r):
@@ -157,7 +112,7 @@ def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: tor
             raise ValueError("scales: no gradient flows into them, pass them detached")
         scales = scales.detach().to(torch.float32).contiguous()
     for t, what in ((ids, "ids"), (scales, "scales")):
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: on {t.device}, x is on {x.device}")
     ids = L.idx64(ids)
     if L.CHECK_INDEX and n > 0 and not _capturing():
@@ -165,8 +120,11 @@ def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: tor
         if lo < -1 or hi >= k:
             raise IndexError(f"adapter id: out of range [{lo}, {hi}] for {k} adapters (-1: none)")
     L.require_device(x)
+    x, w, a, b = _matrix(x), _matrix(w), a.contiguous(), b.contiguous()
     with on_device_of(x):
-        return _AdaptedProjection.apply(_matrix(x, "x"), _matrix(w, "w"), a.contiguous(), b.contiguous(), ids, scales)
+        if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
+            return _AdaptedProjection.apply(x, w, a, b, ids, scales)
+        return _forward(x, w, a, b, ids, scales, False)[0]
 
 
 class LowRankAdapters(torch.nn.Module):

@@ -1,5 +1,7 @@
 """Refusals of the adapted projection (kge/adapter.py): every check of an argument comes before the
 check of the device, so they are all reached with CPU tensors and no launch."""
+import ctypes
+
 import pytest
 import torch
 
@@ -56,11 +58,18 @@ def test_a_new_adapter_changes_nothing_and_scales_follow_alpha():
 
 def test_c_entries_refuse_bad_shapes_without_a_device():
     lib = L.lib()
-    assert lib.kge_adapter_plan(None, 4, 3, None, None, None, None) == 1001
-    assert lib.kge_adapter_shrink(None, 2, 8, 4, 8, None, 1, 3, 2, None, None, None, None, 0, None) == 1001
-    assert lib.kge_adapter_shrink(None, 0, 7, 4, 8, None, 1, 3, 2, None, None, None, None, 0, None) == 1001
-    assert lib.kge_adapter_project(None, 0, 8, 4, 8, None, 8, 6, None, 0, 3, 2, None, None, None, None, 6, None) == 1001
-    assert lib.kge_adapter_grads(None, 0, 8, 4, 8, None, 3, 2000, None, None, None, 0, None, 0, None) == 1001
-    assert lib.kge_adapter_grads_ws_size(4, 8, 3, 2, 2) == 0
-    assert lib.kge_transpose(None, 0, 8, 4, 8, None, 4, None) == 1001
-    assert lib.kge_transpose(None, 0, 8, 0, 8, None, 4, None) == 0
+    assert lib.kge_adapter_save_size(4, 8, 3, 0) == 0 and lib.kge_adapter_save_size(-1, 8, 3, 2) == 0
+    assert lib.kge_adapter_backward_ws_size(2, 4, 8, 6, 3, 2, 1, 1, 1) == 0
+    size = lib.kge_adapter_save_size(4, 8, 3, 2)
+    save = ctypes.create_string_buffer(size + 16)
+    at = (ctypes.addressof(save) + 15) // 16 * 16
+
+    def forward(dtype=0, ldx=8, d=8, m=6, k=3, r=2, save=at, size=size):
+        return lib.kge_adapter_forward(None, dtype, ldx, 4, d, None, 8, m, None, None, k, r, None, None, None, 6, save, size,
+                                       0, None)
+
+    # null tensors, types, strides, sizes, workspaces: a status, never an exception
+    assert {forward(), forward(dtype=2), forward(ldx=7), forward(m=0), forward(k=0), forward(r=1025),
+            forward(save=None), forward(save=at + 4), forward(size=size - 1)} == {1001}
+    assert lib.kge_adapter_backward(None, 0, 6, 4, 6, None, 8, 8, None, 8, None, None, 3, 2, None, at, size, None, 8, None,
+                                    None, None, 0, None) == 1001

@@ -107,10 +107,11 @@ def test_projection_and_gradients(engine, n, d, m, k, r, ids, pad, offset, dtype
     for name in ("y", "dx", "da", "db"):
         check(got[name], want[name], name)
         assert got[name].dtype == dtype
-    # a run without a gradient, or with some of them, gives the same bits; and so does a second run
+    # a run without a gradient takes the path for few requests where there are few: the same bound
     with torch.no_grad():
         y = engine.adapted_projection(t["x"], t["w"], t["a"], t["b"], i, t["scales"])
-    assert torch.equal(y, got["y"])
+    check(y, want["y"], "y")
+    # a second run gives the same bits
     again = run(engine, t, i, ("a", "b"))
     assert torch.equal(again["da"], got["da"]) and torch.equal(again["db"], got["db"])
     for q in range(k):  # an adapter without rows has a zero gradient
