@@ -86,15 +86,15 @@ __device__ __forceinline__ u32x4 frag_strided(const T* p, int64_t stride, int va
 // thread are in flight at once; a batch of up to PT PU rows is read once.
 constexpr int PT = 1024, PU = 8;
 
-__global__ void __launch_bounds__(PT) plan_kernel(const int64_t* __restrict__ ids, int n, int k,
-                                                  int* __restrict__ perm, int* __restrict__ sid, int* __restrict__ start) {
+__device__ __forceinline__ void plan_group(int g, const int64_t* __restrict__ ids, int n, int k, int* __restrict__ perm,
+                                           int* __restrict__ sid, int* __restrict__ start) {
   __shared__ int red[2][PT / 64], count[PU][PT / 64];
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int x[PU];
   auto load = [&](int i0) {
     int64_t v[PU];
 #pragma unroll
-    for (int u = 0; u < PU; ++u) v[u] = ids[min(i0 + u * PT + tid, n - 1)];
+    for (int u = 0; u < PU; ++u) v[u] = i0 + u * PT < n ? ids[min(i0 + u * PT + tid, n - 1)] : 0;
 #pragma unroll
     for (int u = 0; u < PU; ++u) {
       const int in = v[u] == -1 ? k : (v[u] < 0 || v[u] >= k ? k + 1 : (int)v[u]);
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(PT) plan_kernel(const int64_t* __restrict__ id
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < PU; ++u) {
+      if (i0 + u * PT >= n) break;
       int before = 0, total = 0;
 #pragma unroll
       for (int w = 0; w < PT / 64; ++w) {
@@ -160,19 +161,74 @@ __global__ void __launch_bounds__(PT) plan_kernel(const int64_t* __restrict__ id
   }
 }
 
+// ---- h of one row, 16 ranks, columns [c_lo, c_hi), by one wave ------------------------------------------------
+// The matrix instruction with the same row in all 16 places does the sums; put(q, value) for q < 16 (0 from r on).
+// at: the ranks' rows of A_t, ld apart.
+template <typename T, typename F>
+__device__ __forceinline__ void h_row(const T* __restrict__ xr, const T* __restrict__ at, int c_lo, int c_hi, int64_t ld, int r,
+                                      float sc, int lane, F put) {
+  constexpr int N = Mma<T>::N, KC = Mma<T>::KC, U = 4;
+  const int fr = lane & 15, fs = lane >> 4;
+  const T* ap = at + min(fr, r - 1) * ld + fs * N;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = c_lo; c0 < c_hi; c0 += KC * U) {
+    u32x4 a[U], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * KC;
+      a[u] = frag<T>(ap + c, c_hi - c - fs * N);
+      b[u] = frag<T>(xr + c + fs * N, c_hi - c - fs * N);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) Mma<T>::run(acc, a[u], b[u]);
+  }
+  if (fr == 0)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put(fs * 4 + e, fs * 4 + e < r ? acc[e] * sc : 0.f);
+}
+
+// Workgroups 0 .. groups - 1: the plan; the others: h of four rows each, a quarter of the summed axis per wave (no
+// plan needed).  One launch for both: at 1024 rows, 64 adapters and d = 512 two took 5.3 + 4.9 us.
+template <typename T>
+__global__ void __launch_bounds__(PT) plan_h_kernel(const int64_t* __restrict__ ids, int n, int k, int* __restrict__ perm,
+                                                    int* __restrict__ sid, int* __restrict__ start, int groups,
+                                                    const T* __restrict__ x, int64_t ldx, int d, const T* __restrict__ a, int r,
+                                                    int rp, const float* __restrict__ scales, float* __restrict__ h) {
+  __shared__ float part[PT / 64][16];
+  if ((int)blockIdx.x < groups) {
+    plan_group(blockIdx.x, ids, n, k, perm, sid, start);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = wave & 3;
+  const int64_t row = (int64_t)(blockIdx.x - groups) * 4 + (wave >> 2);
+  const int64_t t = row < n ? ids[row] : -1;
+  const bool live = t >= 0 && t < k;
+  const int each = (d + 4 * Mma<T>::KC - 1) / (4 * Mma<T>::KC) * Mma<T>::KC, c0 = quarter * each;
+  for (int q0 = 0; q0 < rp; q0 += 16) {
+    if (live)
+      h_row<T>(x + row * ldx, a + (t * r + q0) * d, c0, min(d, c0 + each), d, min(16, r - q0), 1.f, lane,
+               [&](int q, float v) { part[wave][q] = v; });
+    __syncthreads();
+    if (live && quarter == 0 && lane < 16)
+      h[row * rp + q0 + lane] = ((part[wave][lane] + part[wave + 1][lane]) + (part[wave + 2][lane] + part[wave + 3][lane])) *
+                                (scales ? scales[t] : 1.f);
+    if (q0 + 16 < rp) __syncthreads();
+  }
+}
+
 // Row chunks of `per` rows, each of one adapter: chunk c of adapter t has the slot
 // start[t] / per + t + c (c < max(1, chunks of t)): distinct, and below n / per + k.
 struct Chunk {
   int t, c, row0, rows, chunks;
 };
 __device__ __forceinline__ Chunk chunk_of(int slot, const int* start, int k, int per) {
-  int lo = 0, hi = k - 1;  // the last t with start[t] / per + t <= slot
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (start[mid] / per + mid <= slot)
-      lo = mid;
-    else
-      hi = mid - 1;
+  // the last t with start[t] / per + t <= slot, 64 candidates at a time (two rounds up to 4096 adapters)
+  int lo = 0, hi = k - 1;
+  while (hi > lo) {
+    const int step = (hi - lo + 64) >> 6, t = lo + (int)(threadIdx.x & 63) * step;
+    const bool ok = t <= hi && start[min(t, k - 1)] / per + t <= slot;
+    lo += (__popcll(__ballot(ok)) - 1) * step;
+    hi = min(hi, lo + step - 1);
   }
   const int s0 = start[lo], s1 = start[lo + 1];
   Chunk ch;
@@ -184,7 +240,7 @@ __device__ __forceinline__ Chunk chunk_of(int slot, const int* start, int k, int
   return ch;  // an unused slot has c >= chunks (or c < 0 before the first)
 }
 
-// ---- shrink: out[i, 0 .. r) = scale_t F_t v_i for the sorted rows i --------------------------------
+// ---- shrink: out[i, 0 .. rp) = scale_t F_t v_i for every row i of an adapter ----------------------------
 // F_t as [r, cols] (BY_RANK) or [cols, r].  grid: slots x rank blocks of 16 x splits of the columns (each
 // split a slab of its own).
 template <typename T, bool BY_RANK>
@@ -192,14 +248,15 @@ __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, in
                                                      const T* __restrict__ f, int k, int r, int rp,
                                                      const float* __restrict__ scales, const int* __restrict__ perm,
                                                      const int* __restrict__ start, int per_split, float* __restrict__ out) {
-  constexpr int N = Mma<T>::N, KC = Mma<T>::KC, UN = 4;
+  constexpr int N = Mma<T>::N, KC = Mma<T>::KC, UN = 8;
   __shared__ f32x4 part[4][64];
   const Chunk ch = chunk_of(blockIdx.x, start, k, 16);
   if (ch.c < 0 || ch.c >= ch.chunks || ch.rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fs = lane >> 4;
   const int q = blockIdx.y * 16 + fr;
   const int c_lo = blockIdx.z * per_split, c_hi = min(cols, c_lo + per_split);
-  const T* vr = v + (int64_t)perm[ch.row0 + min(fr, ch.rows - 1)] * ldv;
+  const int row = perm[ch.row0 + min(fr, ch.rows - 1)];
+  const T* vr = v + (int64_t)row * ldv;
   const int64_t fc = BY_RANK ? 1 : r;
   const T* fp = f + (int64_t)ch.t * r * cols + (int64_t)min(q, r - 1) * (BY_RANK ? cols : 1);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -222,7 +279,7 @@ __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, in
   const int q0 = blockIdx.y * 16 + fs * 4;
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] = q0 + e < r ? acc[e] * sc : 0.f;  // ranks up to rp are zeros
-  float* o = out + (int64_t)blockIdx.z * n * rp + (int64_t)(ch.row0 + fr) * rp + q0;
+  float* o = out + (int64_t)blockIdx.z * n * rp + (int64_t)row * rp + q0;
   *reinterpret_cast<f32x4*>(o) = acc;
 }
 
@@ -240,7 +297,7 @@ __global__ void __launch_bounds__(256) slabs_kernel(f32x4* __restrict__ x, int64
 // bytes of the summed axis; the next stage waits in registers.  One stage instead of two lets four workgroups
 // share a CU, whose phases (loads, products, adapters, stores) overlap: with the short summed axes of embedding
 // tables (512: 8 stages) a tile is latency, not MFMA time.
-constexpr int BM = 128, BN = 128, BKB = 128;  // rows of x, rows of W, bytes of the summed axis per stage
+constexpr int BN = 128, BKB = 128;  // rows of W (columns of y), bytes of the summed axis per stage
 
 // 16-byte slot of a 128-byte row, XOR-ed with the row: the 16 rows a fragment read touches then lie in
 // eight different slots
@@ -270,7 +327,7 @@ __device__ __forceinline__ u32x4 h_frag<__bf16>(const float* h, int q0, int fs) 
 // Adapter slices in LDS: 16 ranks of 128 columns, [column][16 ranks].
 template <typename T>
 struct Slice {
-  static constexpr int ROW = 16 * sizeof(T), BYTES = BN * ROW, COUNT = (BM + BN) * BKB / BYTES;
+  static constexpr int ROW = 16 * sizeof(T), BYTES = BN * ROW;
   // where a lane's part of column `col` starts: the ranks its h fragment holds
   static __device__ __forceinline__ int at(int col, int fs) {
     return col * ROW + (sizeof(T) == 4 ? fs : (fs & 1)) * 16;
@@ -289,97 +346,146 @@ __device__ __forceinline__ bool nonfinite(const u32x4& v, __bf16) {
   return b;
 }
 
-// Copies ranks [q0, q0 + 16) of columns [m0, m0 + 128) of an adapter into its slice; whether anything in it is
-// infinite or NaN.
+// A thread's 16-byte pieces of one slice: ranks [q0, q0 + 16) of columns [m0, m0 + 128) of an adapter.
 template <typename T, bool BY_RANK>
-__device__ __forceinline__ bool stage_slice(const T* ft, int m, int r, int m0, int q0, unsigned char* to) {
-  constexpr int N = Mma<T>::N, P = 16 / N;  // 16-byte pieces per column
-  const int tid = threadIdx.x;
-  bool bad = false;
-#pragma unroll
-  for (int it = 0; it < BN * P / 256; ++it) {
-    const int piece = it * 256 + tid;
+struct Piece {
+  static constexpr int N = Mma<T>::N, P = 16 / N, IT = BN * P / 256;  // pieces per column, per thread
+
+  static __device__ __forceinline__ u32x4 load(const T* ft, int m, int r, int m0, int q0, int it) {
+    const int piece = it * 256 + threadIdx.x;
     if (!BY_RANK) {
-      const int col = piece / P, q = q0 + piece % P * N, c = m0 + col;
-      const u32x4 v = c < m ? frag<T>(ft + (int64_t)c * r + q, r - q) : (u32x4){0u, 0u, 0u, 0u};
-      bad |= nonfinite(v, T());
-      *reinterpret_cast<u32x4*>(to + col * Slice<T>::ROW + piece % P * 16) = v;
+      const int c = m0 + piece / P, q = q0 + piece % P * N;
+      return c < m ? frag<T>(ft + (int64_t)c * r + q, r - q) : (u32x4){0u, 0u, 0u, 0u};
+    }
+    const int q = q0 + piece / (BN / N), c = m0 + piece % (BN / N) * N;
+    return q < r ? frag<T>(ft + (int64_t)q * m + c, m - c) : (u32x4){0u, 0u, 0u, 0u};
+  }
+  static __device__ __forceinline__ void store(unsigned char* to, int it, const u32x4& v) {
+    const int piece = it * 256 + threadIdx.x;
+    if (!BY_RANK) {
+      *reinterpret_cast<u32x4*>(to + piece / P * Slice<T>::ROW + piece % P * 16) = v;
     } else {
       typedef T vec __attribute__((ext_vector_type(N)));
-      const int q = piece / (BN / N), col = piece % (BN / N) * N, c = m0 + col;
-      const u32x4 v = q0 + q < r ? frag<T>(ft + (int64_t)(q0 + q) * m + c, m - c) : (u32x4){0u, 0u, 0u, 0u};
-      bad |= nonfinite(v, T());
       const vec x = __builtin_bit_cast(vec, v);
+      const int q = piece / (BN / N), col = piece % (BN / N) * N;
 #pragma unroll
       for (int e = 0; e < N; ++e) *reinterpret_cast<T*>(to + (col + e) * Slice<T>::ROW + q * sizeof(T)) = x[e];
     }
   }
-  return bad;
-}
+};
 
-template <typename T, bool BY_RANK>
-__global__ void __launch_bounds__(256, 3) project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d,
-                                                         const T* __restrict__ w, int64_t ldw, int m,
-                                                         const T* __restrict__ f, int k, int r, int rp,
-                                                         const float* __restrict__ h, const int* __restrict__ perm,
-                                                         const int* __restrict__ sid, T* __restrict__ y, int64_t ldy,
-                                                         int row_tiles, int yvec) {
+// BM 128: the tile above; BM 64: half of its rows, where 128-row tiles leave CUs without work.
+template <typename T, bool BY_RANK, int BM, int STAGES>
+__global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 3)
+    project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, const T* __restrict__ w, int64_t ldw, int m,
+                   const T* __restrict__ f, int k, int r, int rp, const float* __restrict__ h, const int* __restrict__ perm,
+                   const int* __restrict__ sid, T* __restrict__ y, int64_t ldy, int row_tiles, int yvec) {
   constexpr int N = Mma<T>::N, KE = BKB / sizeof(T), KC = Mma<T>::KC;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[(BM + BN) * BKB];
+  constexpr int XP = BM / 32, TM = BM / 32;  // pieces of x per thread and stage; 16-row fragments per wave
+  constexpr int STAGE = (BM + BN) * BKB, LDS = STAGES * STAGE > 32768 ? STAGES * STAGE : 32768;
+  using PC = Piece<T, BY_RANK>;
+  constexpr int COUNT = 8 / PC::IT;  // slices in LDS (and in registers, on their way) at a time: 32 KiB
+  static_assert(COUNT * Slice<T>::BYTES <= LDS, "slices");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
   __shared__ int owner[BM];
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fs = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1;
   const int tile = xcd_remap(blockIdx.x, gridDim.x);
   const int m0 = (tile / row_tiles) * BN, n0 = (tile % row_tiles) * BM;
 
-  const T* src[8];
+  const T* src[XP + 4];
   const int kt = (tid & 7) * N;  // first column of this thread's pieces within a stage
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int row = (tid >> 3) + (j & 3) * 32;
-    if (j < 4)
+  for (int j = 0; j < XP + 4; ++j) {
+    const int row = (tid >> 3) + j * 32;
+    if (j < XP)
       src[j] = x + (int64_t)perm[min(n0 + row, n - 1)] * ldx + kt;
     else
-      src[j] = w + (int64_t)min(m0 + row, m - 1) * ldw + kt;
+      src[j] = w + (int64_t)min(m0 + row - BM, m - 1) * ldw + kt;
   }
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
   u32x4 reg[8];
   auto load = [&](int k0) {  // a whole stage
 #pragma unroll
-    for (int j = 0; j < 8; ++j) __builtin_memcpy(&reg[j], src[j] + k0, 16);
+    for (int j = 0; j < XP + 4; ++j) __builtin_memcpy(&reg[j], src[j] + k0, 16);
   };
   if (KE <= d) load(0);
+
+  // The tile's adapters: sorted rows, so each is a run; slot = its number within the tile (-1: no adapter).
+  const int t_lo = n0 + lane < n ? sid[n0 + lane] : k;
+  const int t_hi = BM == 128 && n0 + 64 + lane < n ? sid[n0 + 64 + lane] : k;
+  const int p_lo = __shfl_up(t_lo, 1, 64), p_hi = __shfl_up(t_hi, 1, 64), mid = __shfl(t_lo, 63, 64);
+  const uint64_t b_lo = __ballot(t_lo < k && (lane == 0 || p_lo != t_lo));
+  const uint64_t b_hi = __ballot(t_hi < k && (lane == 0 ? mid : p_hi) != t_hi);
+  const uint64_t upto = lane == 63 ? ~0ull : (2ull << lane) - 1;
+  const int slot_lo = t_lo < k ? __popcll(b_lo & upto) - 1 : -1;
+  const int slot_hi = t_hi < k ? __popcll(b_lo) + __popcll(b_hi & upto) - 1 : -1;
+  const int slots = __popcll(b_lo) + __popcll(b_hi);
+  if (wave == 0) {
+    if ((b_lo >> lane) & 1) owner[slot_lo] = t_lo;
+    if (BM == 128 && ((b_hi >> lane) & 1)) owner[slot_hi] = t_hi;
+  }
+  // slot (or k + 1: an id out of range) of row `lane` of the half of the tile that this wave's rows lie in
+  const int half = BM == 128 ? wr : 0, lane0 = BM == 128 ? 0 : wr * 32;
+  const int mark = (half ? t_hi : t_lo) > k ? -2 : (half ? slot_hi : slot_lo);
+
+  f32x4 acc[TM][4];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  // slices s0 .. of ranks q0 .. on their way into registers; then into LDS: whether any value is infinite or NaN
+  auto fetch = [&](int q0, int s0) {
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s) {
+      if (s0 + s >= slots) break;
+      const T* ft = f + (int64_t)__builtin_amdgcn_readfirstlane(owner[s0 + s]) * r * m;
+#pragma unroll
+      for (int it = 0; it < PC::IT; ++it) reg[s * PC::IT + it] = PC::load(ft, m, r, m0, q0, it);
+    }
+  };
+  auto put = [&](int s0) {
+    bool bad = false;
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s) {
+      if (s0 + s >= slots) break;
+#pragma unroll
+      for (int it = 0; it < PC::IT; ++it) {
+        bad |= nonfinite(reg[s * PC::IT + it], T());
+        PC::store(lds + s * Slice<T>::BYTES, it, reg[s * PC::IT + it]);
+      }
+    }
+    return bad;
+  };
+
+  int at = 0;  // the stage being filled
   for (int k0 = 0; k0 < d; k0 += KE) {
-    if (k0) __syncthreads();  // the previous stage has been read
+    if (STAGES == 1 && k0) __syncthreads();  // the stage has been read (of two, the barrier below has seen to it)
     if (k0 + KE <= d) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = (tid >> 3) + (j & 3) * 32 + (j < 4 ? 0 : BM);
-        *reinterpret_cast<u32x4*>(&lds[lds_slot(row, tid & 7)]) = reg[j];
-      }
+      for (int j = 0; j < XP + 4; ++j)
+        *reinterpret_cast<u32x4*>(&lds[at + lds_slot((tid >> 3) + j * 32, tid & 7)]) = reg[j];
     } else {  // the rest of the summed axis, zeros behind it
 #pragma unroll 1
       for (int row = tid >> 3; row < BM + BN; row += 32) {
         const T* p = row < BM ? x + (int64_t)perm[min(n0 + row, n - 1)] * ldx : w + (int64_t)min(m0 + row - BM, m - 1) * ldw;
-        *reinterpret_cast<u32x4*>(&lds[lds_slot(row, tid & 7)]) = frag<T>(p + kt + k0, d - k0 - kt);
+        *reinterpret_cast<u32x4*>(&lds[at + lds_slot(row, tid & 7)]) = frag<T>(p + kt + k0, d - k0 - kt);
       }
     }
     __syncthreads();
-    if (k0 + 2 * KE <= d) load(k0 + KE);
+    if (k0 + 2 * KE <= d)
+      load(k0 + KE);
+    else if (k0 + KE >= d)
+      fetch(0, 0);  // behind the last stage's products
 #pragma unroll
     for (int kc = 0; kc < KE / KC; ++kc) {
       u32x4 wb[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        wb[j] = *reinterpret_cast<const u32x4*>(&lds[lds_slot(BM + wc * 64 + j * 16 + fr, kc * 4 + fs)]);
+        wb[j] = *reinterpret_cast<const u32x4*>(&lds[at + lds_slot(BM + wc * 64 + j * 16 + fr, kc * 4 + fs)]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4 xa = *reinterpret_cast<const u32x4*>(&lds[lds_slot(wr * 64 + i * 16 + fr, kc * 4 + fs)]);
+      for (int i = 0; i < TM; ++i) {
+        const u32x4 xa = *reinterpret_cast<const u32x4*>(&lds[at + lds_slot(wr * (BM / 2) + i * 16 + fr, kc * 4 + fs)]);
         if constexpr (sizeof(T) == 4) {  // the four instructions on one accumulator four apart
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -393,62 +499,50 @@ __global__ void __launch_bounds__(256, 3) project_kernel(const T* __restrict__ x
         }
       }
     }
+    if (STAGES == 2) at = STAGE - at;
   }
 
-  // acc[i][j]: x row n0 + wr 64 + i 16 + fr, columns m0 + wc 64 + j 16 + 4 fs + reg.
-  // The tile's adapters: sorted rows, so each is a run; slot = its number within the tile (-1: no adapter).
-  const int t_lo = n0 + lane < n ? sid[n0 + lane] : k, t_hi = n0 + 64 + lane < n ? sid[n0 + 64 + lane] : k;
-  const int p_lo = __shfl_up(t_lo, 1, 64), p_hi = __shfl_up(t_hi, 1, 64), mid = __shfl(t_lo, 63, 64);
-  const uint64_t b_lo = __ballot(t_lo < k && (lane == 0 || p_lo != t_lo));
-  const uint64_t b_hi = __ballot(t_hi < k && (lane == 0 ? mid : p_hi) != t_hi);
-  const uint64_t upto = lane == 63 ? ~0ull : (2ull << lane) - 1;
-  const int slot_lo = t_lo < k ? __popcll(b_lo & upto) - 1 : -1;
-  const int slot_hi = t_hi < k ? __popcll(b_lo) + __popcll(b_hi & upto) - 1 : -1;
-  const int slots = __popcll(b_lo) + __popcll(b_hi);
-  if (wave == 0) {
-    if ((b_lo >> lane) & 1) owner[slot_lo] = t_lo;
-    if ((b_hi >> lane) & 1) owner[slot_hi] = t_hi;
-  }
-  const int slot = wr ? slot_hi : slot_lo, t_own = wr ? t_hi : t_lo;  // of row wr 64 + lane
-
-  if (slots > 0) {
-    for (int q0 = 0; q0 < rp; q0 += 16) {
-      u32x4 hf[4];
+  // acc[i][j]: x row n0 + wr BM / 2 + i 16 + fr, columns m0 + wc 64 + j 16 + 4 fs + reg
+  int from[TM];  // the rows' places in x, h and y
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        hf[i] = h_frag<T>(h + (int64_t)min(n0 + wr * 64 + i * 16 + fr, n - 1) * rp, q0, fs);
-      for (int s0 = 0; s0 < slots; s0 += Slice<T>::COUNT) {
-        const int count = min(Slice<T>::COUNT, slots - s0);
-        __syncthreads();  // the last stage or slices have been read, owner is written
-        bool bad = false;
-#pragma unroll 4
-        for (int s = 0; s < count; ++s)
-          bad |= stage_slice<T, BY_RANK>(f + (int64_t)owner[s0 + s] * r * m, m, r, m0, q0, lds + s * Slice<T>::BYTES);
-        const bool apart = __syncthreads_or(bad);
+  for (int i = 0; i < TM; ++i) from[i] = perm[min(n0 + wr * (BM / 2) + i * 16 + fr, n - 1)];
+  u32x4 hf[TM];
+  for (int q0 = 0, s0 = 0; slots > 0 && q0 < rp;) {
+    if (s0 == 0)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int si = __shfl(slot, i * 16 + fr, 64);
-          const int first = __builtin_amdgcn_readlane(slot, i * 16), end = __builtin_amdgcn_readlane(slot, i * 16 + 15);
-          if (first < 0) continue;  // no adapter from this row on
-          const int last = min(end < 0 ? slots - 1 : end, s0 + count - 1);
-          for (int s = max(first, s0); s <= last; ++s) {
-            const unsigned char* sl = lds + (s - s0) * Slice<T>::BYTES;
-            const bool own = si == s;
-            u32x4 hm;
+      for (int i = 0; i < TM; ++i) hf[i] = h_frag<T>(h + (int64_t)from[i] * rp, q0, fs);
+    __syncthreads();  // the last stage or slices have been read
+    const bool apart = __syncthreads_or(put(s0));
+    const int s_now = s0;
+    s0 += COUNT;
+    if (s0 >= slots) {
+      s0 = 0;
+      q0 += 16;
+    }
+    if (q0 < rp) fetch(q0, s0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hm[e] = own ? hf[i][e] : 0u;
-            if (!apart) {
+    for (int i = 0; i < TM; ++i) {
+      const int si = __shfl(mark, lane0 + i * 16 + fr, 64);
+      const int first = __builtin_amdgcn_readlane(mark, lane0 + i * 16);
+      const int end = __builtin_amdgcn_readlane(mark, lane0 + i * 16 + 15);
+      if (first < 0) continue;  // no adapter from this row on
+      const int last = min(end < 0 ? slots - 1 : end, s_now + COUNT - 1);
+      for (int s = max(first, s_now); s <= last; ++s) {
+        const unsigned char* sl = lds + (s - s_now) * Slice<T>::BYTES;
+        const bool own = si == s;
+        u32x4 hm;
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                Mma<T>::run(acc[i][j], *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
-            } else {  // an infinity times another row's 0 must not reach that row
+        for (int e = 0; e < 4; ++e) hm[e] = own ? hf[i][e] : 0u;
+        if (!apart) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                f32x4 next = acc[i][j];  // the same sum in the same order for the adapter's own rows
-                Mma<T>::run(next, *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
-                if (own) acc[i][j] = next;
-              }
-            }
+          for (int j = 0; j < 4; ++j)
+            Mma<T>::run(acc[i][j], *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
+        } else {  // an infinity times another row's 0 must not reach that row
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4 next = acc[i][j];  // the same sum in the same order for the adapter's own rows
+            Mma<T>::run(next, *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
+            if (own) acc[i][j] = next;
           }
         }
       }
@@ -456,11 +550,10 @@ __global__ void __launch_bounds__(256, 3) project_kernel(const T* __restrict__ x
   }
 
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = n0 + wr * 64 + i * 16 + fr;
-    const float poison = __shfl(t_own, i * 16 + fr, 64) > k ? NAN : 0.f;  // an id out of range
-    if (row >= n) continue;
-    T* yr = y + (int64_t)perm[row] * ldy;
+  for (int i = 0; i < TM; ++i) {
+    const float poison = __shfl(mark, lane0 + i * 16 + fr, 64) == -2 ? NAN : 0.f;  // an id out of range
+    if (n0 + wr * (BM / 2) + i * 16 + fr >= n) continue;
+    T* yr = y + (int64_t)from[i] * ldy;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = m0 + wc * 64 + j * 16 + fs * 4;
@@ -480,35 +573,21 @@ __global__ void __launch_bounds__(256, 3) project_kernel(const T* __restrict__ x
 }
 
 // ---- few requests (serving): unsorted, no plan --------------------------------------------------------------
-// h_i of row i, ranks wave, wave + 4, .. by one wave each, to put(q, value)
-template <typename T, typename F>
-__device__ __forceinline__ void shrink_row(const T* __restrict__ xr, const T* __restrict__ at, int d, int r, float sc, int wave,
-                                           int lane, F put) {
-  constexpr int N = Mma<T>::N;
-  typedef T vec __attribute__((ext_vector_type(N)));
-  for (int q = wave; q < r; q += 4) {
-    float a = 0.f;
-    for (int c = lane * N; c < d; c += 64 * N) {
-      const vec u = __builtin_bit_cast(vec, frag<T>(xr + c, d - c));
-      const vec v = __builtin_bit_cast(vec, frag<T>(at + (int64_t)q * d + c, d - c));
-#pragma unroll
-      for (int e = 0; e < N; ++e) a = fmaf((float)u[e], (float)v[e], a);
-    }
-    a = wave_sum(a);
-    if (lane == 0) put(q, a * sc);
-  }
-}
-
+// (four waves per SIMD: with more registers than it needs hipcc keeps the accumulator in AGPRs and reads it back
+// without the wait its last matrix instruction needs; tests/test_mfma_waits.py checks every build)
 template <typename T>
-__global__ void __launch_bounds__(256) shrink_few_kernel(const T* __restrict__ x, int64_t ldx, int d, const T* __restrict__ a,
-                                                         int k, int r, int rp, const int64_t* __restrict__ ids,
-                                                         const float* __restrict__ scales, float* __restrict__ h) {
-  const int row = blockIdx.x;
+__global__ void __launch_bounds__(256, 4) h_few_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, const T* __restrict__ a,
+                                                    int k, int r, int rp, const int64_t* __restrict__ ids,
+                                                    const float* __restrict__ scales, float* __restrict__ h) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= n) return;
   const int64_t t = ids[row];
   if (t < 0 || t >= k) return;
-  float* hr = h + (int64_t)row * rp;
-  shrink_row<T>(x + row * ldx, a + t * r * d, d, r, scales ? scales[t] : 1.f, threadIdx.x >> 6, threadIdx.x & 63,
-                [&](int q, float v) { hr[q] = v; });
+  for (int q0 = 0; q0 < rp; q0 += 16) {
+    float* hr = h + (int64_t)row * rp + q0;
+    h_row<T>(x + row * ldx, a + (t * r + q0) * d, 0, d, d, min(16, r - q0), scales ? scales[t] : 1.f, threadIdx.x & 63,
+             [&](int q, float v) { hr[q] = v; });
+  }
 }
 
 // A workgroup: 16 columns of y for up to 16 RB rows, its four waves a quarter of the summed axis each; then one
@@ -534,8 +613,8 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
   f32x4 acc[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) acc[rb] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int c0 = wave * KC; c0 < d; c0 += 4 * KC * U) {
-    u32x4 wf[U], xf[U][RB];
+  u32x4 wf[U], xf[U][RB];
+  auto load = [&](int c0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = c0 + u * 4 * KC;
@@ -543,18 +622,24 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) xf[u][rb] = frag<T>(xp[rb] + c, d - c - fs * N);
     }
+  };
+  load(wave * KC);
+  if (INLINE)  // while the first loads are on their way: one wave per (row, 16 ranks)
+    for (int u = wave; u < n * (rp / 16); u += 4) {
+      const int i = u / (rp / 16), q0 = u % (rp / 16) * 16;
+      const int64_t t = ids[i];
+      if (t >= 0 && t < k)
+        h_row<T>(x + i * ldx, a + (t * r + q0) * d, 0, d, d, min(16, r - q0), scales ? scales[t] : 1.f, lane,
+                 [&](int q, float v) { hs[i * rp + q0 + q] = v; });
+    }
+  for (int c0 = wave * KC; c0 < d;) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) Mma<T>::run(acc[rb], wf[u], xf[u][rb]);
+    c0 += 4 * KC * U;
+    if (c0 < d) load(c0);
   }
-  if (INLINE)
-    for (int i = 0; i < n; ++i) {
-      const int64_t t = ids[i];
-      if (t >= 0 && t < k)
-        shrink_row<T>(x + i * ldx, a + t * r * d, d, r, scales ? scales[t] : 1.f, wave, lane,
-                      [&](int q, float v) { hs[i * rp + q] = v; });
-    }
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) part[wave][rb][lane] = acc[rb];
   __syncthreads();
@@ -583,71 +668,117 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
   }
 }
 
-// ---- grads: out_t[q, c] = sum over the sorted rows i of adapter t of h[i, q] v[perm[i], c] -------------
+// ---- grads: out_t[q, c] = sum over the rows i of adapter t of h[i, q] v[i, c] ---------------------------
 // One wave: 16 ranks x 16 N columns (a lane's 16 bytes of a row of v feed N instructions); the four
-// waves of a workgroup take every fourth group of four rows.  Adapters with more than `per` rows are cut into
-// chunks that write fp32 slabs, summed afterwards in ascending order.  An adapter without rows gets zeros.
+// waves of a workgroup take every fourth group of four rows, GU groups on their way at once.  Adapters with more
+// than `per` rows are cut into chunks that write fp32 slabs, summed afterwards in ascending order.  An adapter without
+// rows gets zeros.  Both gradients (dA from x and u, dB from dy and h) in one launch.
 template <typename T>
-__global__ void __launch_bounds__(256) grads_kernel(const T* __restrict__ v, int64_t ldv, int n, int cols,
-                                                    const float* __restrict__ h, int rp, int k, int r,
-                                                    const int* __restrict__ perm, const int* __restrict__ start, int per,
-                                                    T* __restrict__ out, int64_t oc, int64_t oq, float* __restrict__ slabs) {
+struct Grad {
+  const T* v;
+  int64_t ldv;
+  int cols, blocks;  // blocks: of 16 N columns
+  const float* h;
+  T* out;
+  int64_t oc, oq;  // strides of out's columns and ranks
+  float* slabs;
+};
+constexpr int GU = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(256) grads_kernel(Grad<T> g0, Grad<T> g1, int rp, int k, int r,
+                                                    const int* __restrict__ perm, const int* __restrict__ start, int per) {
   constexpr int N = Mma<T>::N;
   typedef T vec __attribute__((ext_vector_type(N)));
-  __shared__ f32x4 part[3][N][64];
+  __shared__ f32x4 part[4][N][64];
   const Chunk ch = chunk_of(blockIdx.x, start, k, per);
   if (ch.c < 0 || ch.c >= ch.chunks) return;
+  const bool second = (int)blockIdx.y >= g0.blocks;
+  const T* __restrict__ v = second ? g1.v : g0.v;
+  const float* __restrict__ h = second ? g1.h : g0.h;
+  const int64_t ldv = second ? g1.ldv : g0.ldv;
+  const int cols = second ? g1.cols : g0.cols, block = second ? blockIdx.y - g0.blocks : blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fs = lane >> 4;
-  const int c0 = blockIdx.y * 16 * N + fr * N, q0 = blockIdx.z * 16;
+  const int c0 = block * 16 * N + fr * N, q0 = blockIdx.z * 16;
   f32x4 acc[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int i = wave * 4; i < ch.rows; i += 16) {
-    const bool in = i + fs < ch.rows;
-    const int row = ch.row0 + min(i + fs, ch.rows - 1);
-    const float hv = in ? h[(int64_t)row * rp + q0 + fr] : 0.f;
-    const vec x = __builtin_bit_cast(vec, frag<T>(v + (int64_t)perm[row] * ldv + c0, in ? cols - c0 : 0));
+  for (int i0 = wave * 4; i0 < ch.rows; i0 += 16 * GU) {
+    int row[GU];
+    float hv[GU];
+    u32x4 x[GU];
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv, (float)x[j], acc[j], 0, 0, 0);
+    for (int u = 0; u < GU; ++u) row[u] = perm[ch.row0 + min(i0 + u * 16 + fs, ch.rows - 1)];
+#pragma unroll
+    for (int u = 0; u < GU; ++u) {
+      const bool in = i0 + u * 16 + fs < ch.rows;
+      hv[u] = in ? h[(int64_t)row[u] * rp + q0 + fr] : 0.f;
+      x[u] = frag<T>(v + (int64_t)row[u] * ldv + c0, in ? cols - c0 : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < GU; ++u) {
+      const vec xv = __builtin_bit_cast(vec, x[u]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[u], (float)xv[j], acc[j], 0, 0, 0);
+    }
   }
-  if (wave > 0)
 #pragma unroll
-    for (int j = 0; j < N; ++j) part[wave - 1][j][lane] = acc[j];
+  for (int j = 0; j < N; ++j) part[wave][j][lane] = acc[j];
   __syncthreads();
-  if (wave > 0) return;
+  // each wave sums and stores a quarter of the columns: ranks q0 + 4 fs + e of columns c0 + J wave + j
+  constexpr int J = N / 4;
+  const int q = q0 + fs * 4, cw = c0 + J * wave;
+  f32x4 sum[J];
 #pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = (acc[j] + part[0][j][lane]) + (part[1][j][lane] + part[2][j][lane]);
-  // acc[j][e]: rank q0 + 4 fs + e, column c0 + j
+  for (int j = 0; j < J; ++j) {
+    const int z = J * wave + j;
+    sum[j] = (part[0][z][lane] + part[1][z][lane]) + (part[2][z][lane] + part[3][z][lane]);
+  }
   if (ch.chunks > 1) {
-    float* sl = slabs + (int64_t)blockIdx.x * r * cols;  // [r][cols]
+    float* sl = (second ? g1.slabs : g0.slabs) + (int64_t)blockIdx.x * r * cols;  // [r][cols]
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (q0 + fs * 4 + e < r && c0 + j < cols) sl[(int64_t)(q0 + fs * 4 + e) * cols + c0 + j] = acc[j][e];
+      for (int j = 0; j < J; ++j)
+        if (q + e < r && cw + j < cols) sl[(int64_t)(q + e) * cols + cw + j] = sum[j][e];
     return;
   }
-  T* o = out + (int64_t)ch.t * r * cols;
+  T* o = (second ? g1.out : g0.out) + (int64_t)ch.t * r * cols;
+  const int64_t oc = second ? g1.oc : g0.oc, oq = second ? g1.oq : g0.oq;
+  typedef T quad __attribute__((ext_vector_type(4)));
+  if (oq == 1 && r % 4 == 0) {  // dB: four ranks of a column side by side
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      quad v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)sum[j][e];
+      if (q < r && cw + j < cols) *reinterpret_cast<quad*>(o + (int64_t)(cw + j) * oc + q) = v;
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (q0 + fs * 4 + e < r && c0 + j < cols) o[(int64_t)(c0 + j) * oc + (int64_t)(q0 + fs * 4 + e) * oq] = (T)acc[j][e];
+    for (int j = 0; j < J; ++j)
+      if (q + e < r && cw + j < cols) o[(int64_t)(cw + j) * oc + (int64_t)(q + e) * oq] = (T)sum[j][e];
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) grads_join_kernel(const float* __restrict__ slabs, const int* __restrict__ start,
-                                                         int per, int cols, int r, T* __restrict__ out, int64_t oc,
-                                                         int64_t oq) {
+__global__ void __launch_bounds__(256) grads_join_kernel(Grad<T> g0, Grad<T> g1, const int* __restrict__ start, int per, int r) {
   const int t = blockIdx.x;
   const int s0 = start[t], chunks = (start[t + 1] - s0 + per - 1) / per;
   if (chunks <= 1) return;
-  const int64_t size = (int64_t)r * cols, slot = s0 / per + t;
-  for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.y * 256) {
-    float a = 0.f;
-    for (int c = 0; c < chunks; ++c) a += slabs[(slot + c) * size + i];
-    const int64_t q = i / cols, col = i - q * cols;
-    out[t * size + col * oc + q * oq] = (T)a;
+  const int64_t slot = s0 / per + t;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const Grad<T>& g = w ? g1 : g0;
+    const int64_t size = (int64_t)r * g.cols;
+    for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.y * 256) {
+      float a = 0.f;
+      for (int c = 0; c < chunks; ++c) a += g.slabs[(slot + c) * size + i];
+      const int64_t q = i / g.cols, col = i - q * g.cols;
+      g.out[t * size + col * g.oc + q * g.oq] = (T)a;
+    }
   }
 }
 
@@ -671,6 +802,10 @@ bool dtype_ok(int dtype) { return dtype == KGE_DT_F32 || dtype == KGE_DT_BF16; }
 bool ld_ok(int64_t ld, int64_t rows, int64_t cols) { return rows <= 1 || ld >= cols; }
 constexpr int64_t MAX_N = (int64_t)1 << 30, MAX_K = 1 << 20, MAX_R = 1024;
 constexpr int64_t FEW = 32;  // rows of the serving path
+#ifndef PSMALL
+#define PSMALL 2
+#endif
+constexpr int64_t PROJECT_SMALL = PSMALL;
 int64_t rank_pad(int64_t r) { return (r + 15) / 16 * 16; }
 int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -697,16 +832,15 @@ int shrink_splits(int64_t n, int64_t cols, int64_t k, int64_t rp) {
   return (int)std::max<int64_t>(1, std::min(want, most));
 }
 
-// Rows of one chunk of grads: at least 256 (16 rounds of a workgroup), so that few adapters need their
+// Rows of one chunk of grads: at least 1024 (16 rounds of a workgroup), so that few adapters need their
 // chunks joined; more where the launch would exceed about 2048 workgroups
 int64_t grads_per(int64_t n, int64_t cols, int64_t r, int es) {
-  const int64_t blocks = ((cols * es + 255) / 256) * (rank_pad(r) / 16);
+  const int64_t blocks = std::max<int64_t>(1, (cols * es + 255) / 256) * (rank_pad(r) / 16);  // (cols 0: no gradient wanted)
   const int64_t chunks = std::max<int64_t>(1, 2048 / blocks);
-  return std::max<int64_t>(256, ((n + chunks - 1) / chunks + 63) / 64 * 64);
+  return std::max<int64_t>(1024, ((n + chunks - 1) / chunks + 63) / 64 * 64);
 }
-int64_t grads_ws(int64_t n, int64_t cols, int64_t k, int64_t r, int es) {
-  const int64_t per = grads_per(n, cols, r, es);
-  return n <= per ? 0 : (n / per + k) * r * cols * 4;
+int64_t grads_ws(int64_t n, int64_t cols, int64_t k, int64_t r, int64_t per) {
+  return n <= per ? 0 : round256((n / per + k) * r * cols * 4);
 }
 
 // what the forward pass leaves for the backward one: the plan and h
@@ -735,7 +869,8 @@ struct BackWs {
   float* u;
   void* wt;
   int64_t ldwt;
-  float* slabs;
+  int64_t per;
+  float *slabs_a, *slabs_b;
   int64_t bytes;
 };
 BackWs back_ws_of(void* base, int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r, bool dx, bool da, bool db) {
@@ -748,16 +883,30 @@ BackWs back_ws_of(void* base, int dtype, int64_t n, int64_t d, int64_t m, int64_
   s.ldwt = (m * es + 15) / 16 * 16 / es;
   s.wt = b + o;
   if (dx) o += round256(d * s.ldwt * es);
-  s.slabs = (float*)(b + o);
-  o += round256(std::max(da ? grads_ws(n, d, k, r, es) : 0, db ? grads_ws(n, m, k, r, es) : 0));
+  s.per = grads_per(n, (da ? d : 0) + (db ? m : 0), r, es);
+  s.slabs_a = (float*)(b + o);
+  if (da) o += grads_ws(n, d, k, r, s.per);
+  s.slabs_b = (float*)(b + o);
+  if (db) o += grads_ws(n, m, k, r, s.per);
   s.bytes = o;
   return s;
 }
 
-int run_plan(const int64_t* ids, int64_t n, int64_t k, const Save& s, hipStream_t st) {
-  plan_kernel<<<dim3((unsigned)(k + 2)), dim3(PT), 0, st>>>(ids, (int)n, (int)k, s.perm, s.sid, s.start);
+// The plan, and h of every row: in the same launch where each row reading its own A_t costs little (24 MiB from
+// the L2s), else by adapter afterwards.
+template <typename T, bool BY_RANK>
+int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int64_t k, int64_t r, const float* scales,
+               const Save& s, float* out, hipStream_t st);
+
+template <typename T>
+int run_plan_h(const int64_t* ids, const T* x, int64_t ldx, int64_t n, int64_t d, const T* a, int64_t k, int64_t r,
+               const float* scales, const Save& s, hipStream_t st) {
+  const bool with_h = n * r * d * (int64_t)sizeof(T) <= 24 << 20;
+  const int64_t groups = k + 2, blocks = groups + (with_h ? (n + 3) / 4 : 0);
+  plan_h_kernel<T><<<dim3((unsigned)blocks), dim3(PT), 0, st>>>(ids, (int)n, (int)k, s.perm, s.sid, s.start, (int)groups, x,
+                                                                ldx, (int)d, a, (int)r, (int)rank_pad(r), scales, s.h);
   KGE_CHECK_LAUNCH();
-  return 0;
+  return with_h || n == 0 ? 0 : run_shrink<T, true>(x, ldx, n, d, a, k, r, scales, s, s.h, st);
 }
 
 template <typename T, bool BY_RANK>
@@ -775,32 +924,43 @@ int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int
   return 0;
 }
 
-template <typename T, bool BY_RANK>
-int run_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
-                int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
+template <typename T, bool BY_RANK, int BM>
+int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
+                   int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
+  // fp32 is bound by its matrix instructions: two workgroups per CU with two stages each keep them fed, and
+  // share the last round of tiles better than three (133 against 105 TFLOP/s at 4096^3)
+  constexpr int STAGES = sizeof(T) == 4 ? 2 : 1;
   const int64_t row_tiles = (n + BM - 1) / BM, tiles = row_tiles * ((m + BN - 1) / BN);
   KGE_REQUIRE(tiles < ((int64_t)1 << 31));
   const int yvec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T))) == 0 && ldy % 4 == 0;
-  project_kernel<T, BY_RANK><<<dim3((unsigned)tiles), dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k,
-                                                                          (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy,
-                                                                          (int)row_tiles, yvec);
+  project_kernel<T, BY_RANK, BM, STAGES><<<dim3((unsigned)tiles), dim3(256), 0, st>>>(
+      x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k, (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy, (int)row_tiles,
+      yvec);
   KGE_CHECK_LAUNCH();
   return 0;
 }
 
+template <typename T, bool BY_RANK>
+int run_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
+                int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
+  const int64_t tiles = ((n + 127) / 128) * ((m + BN - 1) / BN);
+  return tiles < PROJECT_SMALL * kge_num_cus()
+             ? launch_project<T, BY_RANK, 64>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st)
+             : launch_project<T, BY_RANK, 128>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st);
+}
+
 template <typename T>
-int run_grads(const T* v, int64_t ldv, int64_t n, int64_t cols, const float* h, int64_t k, int64_t r, const Save& s, T* out,
-              bool by_rank, float* slabs, hipStream_t st) {
-  const int64_t per = grads_per(n, cols, r, sizeof(T)), blocks = (cols * sizeof(T) + 255) / 256;
-  const int64_t oc = by_rank ? 1 : r, oq = by_rank ? cols : 1;
+int run_grads(Grad<T> g0, Grad<T> g1, int64_t n, int64_t k, int64_t r, const Save& s, int64_t per, hipStream_t st) {
+  g0.blocks = (int)((g0.cols * (int64_t)sizeof(T) + 255) / 256);
+  g1.blocks = (int)((g1.cols * (int64_t)sizeof(T) + 255) / 256);
+  const int64_t blocks = (int64_t)g0.blocks + g1.blocks, cols = (int64_t)g0.cols + g1.cols;
   KGE_REQUIRE(blocks <= 65535);
   grads_kernel<T><<<dim3((unsigned)(n / per + k), (unsigned)blocks, (unsigned)(rank_pad(r) / 16)), dim3(256), 0, st>>>(
-      v, ldv, (int)n, (int)cols, h, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per, out, oc, oq, slabs);
+      g0, g1, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per);
   KGE_CHECK_LAUNCH();
   if (n <= per) return 0;
   const int64_t join = std::max<int64_t>(1, std::min<int64_t>((r * cols + 255) / 256, 64));
-  grads_join_kernel<T><<<dim3((unsigned)k, (unsigned)join), dim3(256), 0, st>>>(slabs, s.start, (int)per, (int)cols, (int)r,
-                                                                                out, oc, oq);
+  grads_join_kernel<T><<<dim3((unsigned)k, (unsigned)join), dim3(256), 0, st>>>(g0, g1, s.start, (int)per, (int)r);
   KGE_CHECK_LAUNCH();
   return 0;
 }
@@ -816,7 +976,8 @@ int run_few(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t l
     KGE_CHECK_LAUNCH();
     return 0;
   }
-  shrink_few_kernel<T><<<dim3((unsigned)n), dim3(256), 0, st>>>(x, ldx, (int)d, a, (int)k, (int)r, rp, ids, scales, h);
+  h_few_kernel<T><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, a, (int)k, (int)r, rp, ids,
+                                                                       scales, h);
   KGE_CHECK_LAUNCH();
   project_few_kernel<T, RB, false><<<grid, dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r,
                                                                rp, ids, scales, h, y, ldy);
@@ -860,9 +1021,8 @@ extern "C" int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_
       return n <= 16 ? run_few<T, 1>(xt, ldx, n, d, wt, ldw, m, at, bt, k, r, ids, scales, s.h, yt, ldy, st)
                      : run_few<T, 2>(xt, ldx, n, d, wt, ldw, m, at, bt, k, r, ids, scales, s.h, yt, ldy, st);
     }
-    KGE_TRY(run_plan(ids, n, k, s, st));
+    KGE_TRY(run_plan_h<T>(ids, xt, ldx, n, d, at, k, r, scales, s, st));
     if (n == 0) return 0;
-    KGE_TRY((run_shrink<T, true>(xt, ldx, n, d, at, k, r, scales, s, s.h, st)));
     return run_project<T, false>(xt, ldx, n, d, wt, ldw, m, bt, k, r, s.h, s, yt, ldy, st);
   });
 }
@@ -892,8 +1052,9 @@ extern "C" int kge_adapter_backward(const void* dy, int dtype, int64_t lddy, int
       KGE_TRY(run_transpose<T>(wt, ldw, m, d, (T*)q.wt, q.ldwt, st));
       KGE_TRY((run_project<T, true>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, at, k, r, q.u, s, (T*)dx, lddx, st)));
     }
-    if (da) KGE_TRY(run_grads<T>(xt, ldx, n, d, q.u, k, r, s, (T*)da, true, q.slabs, st));
-    if (db) KGE_TRY(run_grads<T>(dyt, lddy, n, m, s.h, k, r, s, (T*)db, false, q.slabs, st));
-    return 0;
+    const Grad<T> ga{xt, ldx, (int)d, 0, q.u, (T*)da, 1, d, q.slabs_a}, gb{dyt, lddy, (int)m, 0, s.h, (T*)db, r, 1, q.slabs_b};
+    const Grad<T> none{nullptr, 0, 0, 0, nullptr, nullptr, 0, 0, nullptr};
+    if (!da && !db) return 0;
+    return run_grads<T>(da ? ga : gb, da && db ? gb : none, n, k, r, s, q.per, st);
   });
 }

@@ -60,6 +60,8 @@ def test_c_entries_refuse_bad_shapes_without_a_device():
     lib = L.lib()
     assert lib.kge_adapter_save_size(4, 8, 3, 0) == 0 and lib.kge_adapter_save_size(-1, 8, 3, 2) == 0
     assert lib.kge_adapter_backward_ws_size(2, 4, 8, 6, 3, 2, 1, 1, 1) == 0
+    for want in ((0, 0, 0), (1, 0, 0), (0, 1, 0), (0, 0, 1)):  # any choice of gradients has a size
+        assert lib.kge_adapter_backward_ws_size(0, 4, 8, 6, 3, 2, *want) >= 0
     size = lib.kge_adapter_save_size(4, 8, 3, 2)
     save = ctypes.create_string_buffer(size + 16)
     at = (ctypes.addressof(save) + 15) // 16 * 16
