@@ -22,6 +22,7 @@
 // (2^-16), both halves in one instruction: 16 ranks fill half of its 32-wide summed axis.
 #include <math.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.h"
@@ -53,30 +54,53 @@ struct Mma<float> {
   }
 };
 
-// `valid` (possibly <= 0) consecutive elements of a lane's 16 bytes, the rest 0.  Rows need no alignment beyond
-// their elements' own: the hardware splits a 16-byte load that crosses a line.
-template <typename T>
-__device__ __forceinline__ u32x4 frag(const T* p, int valid) {
+// A lane's 16 bytes: elements off .. of a row of len, zeros from len on (off may lie beyond it).  No branches: a
+// batch of them is in flight together (guarded by branches, each load waits for the one before: the compiler drains
+// the loads where the paths meet).  EVEN: len and off are multiples of N, a fragment lies inside or outside.  Rows need
+// no alignment beyond their elements' own: the hardware splits a load that crosses a line.
+template <typename T, bool EVEN>
+__device__ __forceinline__ u32x4 frag(const T* row, int off, int len) {
   constexpr int N = Mma<T>::N;
-  if (valid >= N) {
-    u32x4 whole;
-    __builtin_memcpy(&whole, p, 16);
-    return whole;
+  u32x4 v;
+  if (EVEN) {
+    const bool in = off < len;
+    __builtin_memcpy(&v, row + (in ? off : 0), 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = in ? v[e] : 0u;
+    return v;
+  }
+  if (len >= N) {  // the row's last N elements where the fragment crosses its end, shifted down
+    const int at = min(off, len - N), s = min(off - at, N) * (int)sizeof(T) * 8;
+    uint64_t q[2];
+    __builtin_memcpy(q, row + at, 16);
+    const uint64_t low = s < 64 ? (q[0] >> s) | (s ? q[1] << (64 - s) : 0) : (s < 128 ? q[1] >> (s - 64) : 0);
+    const uint64_t high = s < 64 ? q[1] >> s : 0;
+    v[0] = (unsigned)low;
+    v[1] = (unsigned)(low >> 32);
+    v[2] = (unsigned)high;
+    v[3] = (unsigned)(high >> 32);
+    return v;
   }
   typedef T vec __attribute__((ext_vector_type(N)));
-  vec v;
+  vec x;
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = e < valid ? p[e] : (T)0.f;
-  return __builtin_bit_cast(u32x4, v);
+  for (int e = 0; e < N; ++e) {
+    const T z = row[min(off + e, len - 1)];
+    x[e] = off + e < len ? z : (T)0.f;
+  }
+  return __builtin_bit_cast(u32x4, x);
 }
-// the same, `stride` elements apart
+// elements off, off + 1, .. of a column: `stride` apart in memory
 template <typename T>
-__device__ __forceinline__ u32x4 frag_strided(const T* p, int64_t stride, int valid) {
+__device__ __forceinline__ u32x4 frag_strided(const T* col, int64_t stride, int off, int len) {
   constexpr int N = Mma<T>::N;
   typedef T vec __attribute__((ext_vector_type(N)));
   vec v;
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = e < valid ? p[e * stride] : (T)0.f;
+  for (int e = 0; e < N; ++e) {
+    const T z = col[min(off + e, len - 1) * stride];
+    v[e] = off + e < len ? z : (T)0.f;
+  }
   return __builtin_bit_cast(u32x4, v);
 }
 
@@ -164,20 +188,20 @@ __device__ __forceinline__ void plan_group(int g, const int64_t* __restrict__ id
 // ---- h of one row, 16 ranks, columns [c_lo, c_hi), by one wave ------------------------------------------------
 // The matrix instruction with the same row in all 16 places does the sums; put(q, value) for q < 16 (0 from r on).
 // at: the ranks' rows of A_t, ld apart.
-template <typename T, typename F>
+template <typename T, bool EVEN, typename F>
 __device__ __forceinline__ void h_row(const T* __restrict__ xr, const T* __restrict__ at, int c_lo, int c_hi, int64_t ld, int r,
                                       float sc, int lane, F put) {
   constexpr int N = Mma<T>::N, KC = Mma<T>::KC, U = 4;
   const int fr = lane & 15, fs = lane >> 4;
-  const T* ap = at + min(fr, r - 1) * ld + fs * N;
+  const T* ap = at + min(fr, r - 1) * ld;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int c0 = c_lo; c0 < c_hi; c0 += KC * U) {
     u32x4 a[U], b[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * KC;
-      a[u] = frag<T>(ap + c, c_hi - c - fs * N);
-      b[u] = frag<T>(xr + c + fs * N, c_hi - c - fs * N);
+      const int c = c0 + u * KC + fs * N;
+      a[u] = frag<T, EVEN>(ap, c, c_hi);
+      b[u] = frag<T, EVEN>(xr, c, c_hi);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) Mma<T>::run(acc, a[u], b[u]);
@@ -189,7 +213,7 @@ __device__ __forceinline__ void h_row(const T* __restrict__ xr, const T* __restr
 
 // Workgroups 0 .. groups - 1: the plan; the others: h of four rows each, a quarter of the summed axis per wave (no
 // plan needed).  One launch for both: at 1024 rows, 64 adapters and d = 512 two took 5.3 + 4.9 us.
-template <typename T>
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(PT) plan_h_kernel(const int64_t* __restrict__ ids, int n, int k, int* __restrict__ perm,
                                                     int* __restrict__ sid, int* __restrict__ start, int groups,
                                                     const T* __restrict__ x, int64_t ldx, int d, const T* __restrict__ a, int r,
@@ -206,7 +230,7 @@ __global__ void __launch_bounds__(PT) plan_h_kernel(const int64_t* __restrict__ 
   const int each = (d + 4 * Mma<T>::KC - 1) / (4 * Mma<T>::KC) * Mma<T>::KC, c0 = quarter * each;
   for (int q0 = 0; q0 < rp; q0 += 16) {
     if (live)
-      h_row<T>(x + row * ldx, a + (t * r + q0) * d, c0, min(d, c0 + each), d, min(16, r - q0), 1.f, lane,
+      h_row<T, EVEN>(x + row * ldx, a + (t * r + q0) * d, c0, min(d, c0 + each), d, min(16, r - q0), 1.f, lane,
                [&](int q, float v) { part[wave][q] = v; });
     __syncthreads();
     if (live && quarter == 0 && lane < 16)
@@ -243,7 +267,7 @@ __device__ __forceinline__ Chunk chunk_of(int slot, const int* start, int k, int
 // ---- shrink: out[i, 0 .. rp) = scale_t F_t v_i for every row i of an adapter ----------------------------
 // F_t as [r, cols] (BY_RANK) or [cols, r].  grid: slots x rank blocks of 16 x splits of the columns (each
 // split a slab of its own).
-template <typename T, bool BY_RANK>
+template <typename T, bool BY_RANK, bool EVEN>
 __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, int64_t ldv, int n, int cols,
                                                      const T* __restrict__ f, int k, int r, int rp,
                                                      const float* __restrict__ scales, const int* __restrict__ perm,
@@ -257,7 +281,6 @@ __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, in
   const int c_lo = blockIdx.z * per_split, c_hi = min(cols, c_lo + per_split);
   const int row = perm[ch.row0 + min(fr, ch.rows - 1)];
   const T* vr = v + (int64_t)row * ldv;
-  const int64_t fc = BY_RANK ? 1 : r;
   const T* fp = f + (int64_t)ch.t * r * cols + (int64_t)min(q, r - 1) * (BY_RANK ? cols : 1);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int c0 = c_lo + wave * KC; c0 < c_hi; c0 += 4 * KC * UN) {
@@ -265,8 +288,8 @@ __global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ v, in
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int c = c0 + u * 4 * KC + fs * N;
-      a[u] = BY_RANK ? frag<T>(fp + c, c_hi - c) : frag_strided<T>(fp + (int64_t)c * fc, fc, c_hi - c);
-      b[u] = frag<T>(vr + c, c_hi - c);
+      a[u] = BY_RANK ? frag<T, EVEN>(fp, c, c_hi) : frag_strided<T>(fp, r, c, c_hi);
+      b[u] = frag<T, EVEN>(vr, c, c_hi);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) Mma<T>::run(acc, a[u], b[u]);
@@ -293,10 +316,15 @@ __global__ void __launch_bounds__(256) slabs_kernel(f32x4* __restrict__ x, int64
 }
 
 // ---- project: y[perm[i], :] = W x + F_t h_i -----------------------------------------------------------
-// F_t as [m, r] or (BY_RANK) [r, m].  128 x 128 tiles, four waves of 64 x 64, one 32-KiB LDS stage of 128
-// bytes of the summed axis; the next stage waits in registers.  One stage instead of two lets four workgroups
-// share a CU, whose phases (loads, products, adapters, stores) overlap: with the short summed axes of embedding
-// tables (512: 8 stages) a tile is latency, not MFMA time.
+// F_t as [m, r].  128 x 128 tiles, four waves of 64 x 64, one 32-KiB LDS stage of 128 bytes of the summed axis
+// (fp32: two); the next stage waits in registers.  One stage instead of two lets three workgroups share a CU, whose
+// phases (loads, products, adapters, stores) overlap: with the short summed axes of embedding tables (512: 8 stages)
+// a bf16 tile is latency, not MFMA time.  The slices of eight adapters at a time come into registers behind the last
+// stage's products and go to where the stage was.
+// 1024 x 14541 x 512, bf16: 30 us without adapters (the traffic of W, x and y needs 9, the products 6), 47 us with 64
+// adapters of rank 16 (30 MB more); fp32: 159 us (96 TFLOP/s) and 172 us with 32 of rank 8.  Tried and slower: all of
+// x's rows of a workgroup in LDS with W straight into registers (32 / 50 us), a walk over tiles by as many workgroups
+// as fit (spills), slices straight into registers (33 / 49 us), twelve slices at a time (spills).
 constexpr int BN = 128, BKB = 128;  // rows of W (columns of y), bytes of the summed axis per stage
 
 // 16-byte slot of a 128-byte row, XOR-ed with the row: the 16 rows a fragment read touches then lie in
@@ -347,43 +375,32 @@ __device__ __forceinline__ bool nonfinite(const u32x4& v, __bf16) {
 }
 
 // A thread's 16-byte pieces of one slice: ranks [q0, q0 + 16) of columns [m0, m0 + 128) of an adapter.
-template <typename T, bool BY_RANK>
+template <typename T, bool EVEN>
 struct Piece {
   static constexpr int N = Mma<T>::N, P = 16 / N, IT = BN * P / 256;  // pieces per column, per thread
 
   static __device__ __forceinline__ u32x4 load(const T* ft, int m, int r, int m0, int q0, int it) {
     const int piece = it * 256 + threadIdx.x;
-    if (!BY_RANK) {
-      const int c = m0 + piece / P, q = q0 + piece % P * N;
-      return c < m ? frag<T>(ft + (int64_t)c * r + q, r - q) : (u32x4){0u, 0u, 0u, 0u};
-    }
-    const int q = q0 + piece / (BN / N), c = m0 + piece % (BN / N) * N;
-    return q < r ? frag<T>(ft + (int64_t)q * m + c, m - c) : (u32x4){0u, 0u, 0u, 0u};
+    return frag<T, EVEN>(ft + (int64_t)min(m0 + piece / P, m - 1) * r, q0 + piece % P * N, r);
   }
   static __device__ __forceinline__ void store(unsigned char* to, int it, const u32x4& v) {
     const int piece = it * 256 + threadIdx.x;
-    if (!BY_RANK) {
-      *reinterpret_cast<u32x4*>(to + piece / P * Slice<T>::ROW + piece % P * 16) = v;
-    } else {
-      typedef T vec __attribute__((ext_vector_type(N)));
-      const vec x = __builtin_bit_cast(vec, v);
-      const int q = piece / (BN / N), col = piece % (BN / N) * N;
-#pragma unroll
-      for (int e = 0; e < N; ++e) *reinterpret_cast<T*>(to + (col + e) * Slice<T>::ROW + q * sizeof(T)) = x[e];
-    }
+    *reinterpret_cast<u32x4*>(to + piece / P * Slice<T>::ROW + piece % P * 16) = v;
   }
 };
 
 // BM 128: the tile above; BM 64: half of its rows, where 128-row tiles leave CUs without work.
-template <typename T, bool BY_RANK, int BM, int STAGES>
-__global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 3)
+// bf16: three workgroups per CU (87 us against two's 92 at 1024 x 14541 x 2048); fragments of odd ranks need the
+// registers of two, or they spill.
+template <typename T, int BM, int STAGES, bool EVEN>
+__global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, const T* __restrict__ w, int64_t ldw, int m,
                    const T* __restrict__ f, int k, int r, int rp, const float* __restrict__ h, const int* __restrict__ perm,
                    const int* __restrict__ sid, T* __restrict__ y, int64_t ldy, int row_tiles, int yvec) {
   constexpr int N = Mma<T>::N, KE = BKB / sizeof(T), KC = Mma<T>::KC;
   constexpr int XP = BM / 32, TM = BM / 32;  // pieces of x per thread and stage; 16-row fragments per wave
   constexpr int STAGE = (BM + BN) * BKB, LDS = STAGES * STAGE > 32768 ? STAGES * STAGE : 32768;
-  using PC = Piece<T, BY_RANK>;
+  using PC = Piece<T, EVEN>;
   constexpr int COUNT = 8 / PC::IT;  // slices in LDS (and in registers, on their way) at a time: 32 KiB
   static_assert(COUNT * Slice<T>::BYTES <= LDS, "slices");
   __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
@@ -469,7 +486,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 3)
 #pragma unroll 1
       for (int row = tid >> 3; row < BM + BN; row += 32) {
         const T* p = row < BM ? x + (int64_t)perm[min(n0 + row, n - 1)] * ldx : w + (int64_t)min(m0 + row - BM, m - 1) * ldw;
-        *reinterpret_cast<u32x4*>(&lds[at + lds_slot(row, tid & 7)]) = frag<T>(p + kt + k0, d - k0 - kt);
+        *reinterpret_cast<u32x4*>(&lds[at + lds_slot(row, tid & 7)]) = frag<T, false>(p, k0 + kt, d);
       }
     }
     __syncthreads();
@@ -575,7 +592,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 3)
 // ---- few requests (serving): unsorted, no plan --------------------------------------------------------------
 // (four waves per SIMD: with more registers than it needs hipcc keeps the accumulator in AGPRs and reads it back
 // without the wait its last matrix instruction needs; tests/test_mfma_waits.py checks every build)
-template <typename T>
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(256, 4) h_few_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, const T* __restrict__ a,
                                                     int k, int r, int rp, const int64_t* __restrict__ ids,
                                                     const float* __restrict__ scales, float* __restrict__ h) {
@@ -585,7 +602,7 @@ __global__ void __launch_bounds__(256, 4) h_few_kernel(const T* __restrict__ x, 
   if (t < 0 || t >= k) return;
   for (int q0 = 0; q0 < rp; q0 += 16) {
     float* hr = h + (int64_t)row * rp + q0;
-    h_row<T>(x + row * ldx, a + (t * r + q0) * d, 0, d, d, min(16, r - q0), scales ? scales[t] : 1.f, threadIdx.x & 63,
+    h_row<T, EVEN>(x + row * ldx, a + (t * r + q0) * d, 0, d, d, min(16, r - q0), scales ? scales[t] : 1.f, threadIdx.x & 63,
              [&](int q, float v) { hr[q] = v; });
   }
 }
@@ -593,7 +610,7 @@ __global__ void __launch_bounds__(256, 4) h_few_kernel(const T* __restrict__ x, 
 // A workgroup: 16 columns of y for up to 16 RB rows, its four waves a quarter of the summed axis each; then one
 // thread per value adds B_t h.  INLINE: h is worked out by every workgroup for itself (a row or two: A_t comes from
 // the L2, and a launch less).
-template <typename T, int RB, bool INLINE>
+template <typename T, int RB, bool INLINE, bool EVEN>
 __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ x, int64_t ldx, int n, int d,
                                                           const T* __restrict__ w, int64_t ldw, int m,
                                                           const T* __restrict__ a, const T* __restrict__ b, int k, int r,
@@ -606,10 +623,10 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
   extern __shared__ float hs[];  // INLINE: [n][rp]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fs = lane >> 4;
   const int m0 = blockIdx.x * 16;
-  const T* wp = w + (int64_t)min(m0 + fr, m - 1) * ldw + fs * N;
+  const T* wp = w + (int64_t)min(m0 + fr, m - 1) * ldw;
   const T* xp[RB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) xp[rb] = x + (int64_t)min(rb * 16 + fr, n - 1) * ldx + fs * N;
+  for (int rb = 0; rb < RB; ++rb) xp[rb] = x + (int64_t)min(rb * 16 + fr, n - 1) * ldx;
   f32x4 acc[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) acc[rb] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -617,10 +634,10 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
   auto load = [&](int c0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * 4 * KC;
-      wf[u] = frag<T>(wp + c, d - c - fs * N);
+      const int c = c0 + u * 4 * KC + fs * N;
+      wf[u] = frag<T, EVEN>(wp, c, d);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) xf[u][rb] = frag<T>(xp[rb] + c, d - c - fs * N);
+      for (int rb = 0; rb < RB; ++rb) xf[u][rb] = frag<T, EVEN>(xp[rb], c, d);
     }
   };
   load(wave * KC);
@@ -629,7 +646,7 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
       const int i = u / (rp / 16), q0 = u % (rp / 16) * 16;
       const int64_t t = ids[i];
       if (t >= 0 && t < k)
-        h_row<T>(x + i * ldx, a + (t * r + q0) * d, 0, d, d, min(16, r - q0), scales ? scales[t] : 1.f, lane,
+        h_row<T, EVEN>(x + i * ldx, a + (t * r + q0) * d, 0, d, d, min(16, r - q0), scales ? scales[t] : 1.f, lane,
                  [&](int q, float v) { hs[i * rp + q0 + q] = v; });
     }
   for (int c0 = wave * KC; c0 < d;) {
@@ -655,7 +672,7 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
       const float* hr = INLINE ? hs + row * rp : h + (int64_t)row * rp;
       float add = 0.f;
       for (int q = 0; q < r; q += N) {
-        const vec bv = __builtin_bit_cast(vec, frag<T>(bt + q, r - q));
+        const vec bv = __builtin_bit_cast(vec, frag<T, EVEN>(bt, q, r));
 #pragma unroll
         for (int z = 0; z < N; ++z)
           if (q + z < r) add = fmaf((float)bv[z], hr[q + z], add);
@@ -685,7 +702,7 @@ struct Grad {
 };
 constexpr int GU = 4;
 
-template <typename T>
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(256) grads_kernel(Grad<T> g0, Grad<T> g1, int rp, int k, int r,
                                                     const int* __restrict__ perm, const int* __restrict__ start, int per) {
   constexpr int N = Mma<T>::N;
@@ -713,7 +730,7 @@ __global__ void __launch_bounds__(256) grads_kernel(Grad<T> g0, Grad<T> g1, int 
     for (int u = 0; u < GU; ++u) {
       const bool in = i0 + u * 16 + fs < ch.rows;
       hv[u] = in ? h[(int64_t)row[u] * rp + q0 + fr] : 0.f;
-      x[u] = frag<T>(v + (int64_t)row[u] * ldv + c0, in ? cols - c0 : 0);
+      x[u] = frag<T, EVEN>(v + (int64_t)row[u] * ldv, in ? c0 : cols, cols);
     }
 #pragma unroll
     for (int u = 0; u < GU; ++u) {
@@ -782,17 +799,37 @@ __global__ void __launch_bounds__(256) grads_join_kernel(Grad<T> g0, Grad<T> g1,
   }
 }
 
-// dst [cols, ldd] = src [rows, lds] transposed, 32 x 32 tiles
+// dst [cols, ldd] = src [rows, lds] transposed, 32 x 32 tiles, for W and (blockIdx.z > 0) every A_t
 template <typename T>
-__global__ void __launch_bounds__(256) transpose_kernel(const T* __restrict__ src, int64_t lds_, int rows, int cols,
-                                                        T* __restrict__ dst, int64_t ldd) {
+struct Flip {
+  const T* src;
+  int64_t lds, src_next;
+  int rows, cols;
+  T* dst;
+  int64_t ldd, dst_next;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) transpose_kernel(Flip<T> w, Flip<T> a, int w_tiles, int w_across, int a_tiles, int a_across) {
   __shared__ T tile[32][33];
-  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  int b = blockIdx.x;
+  const bool first = b < w_tiles;
+  const Flip<T>& z = first ? w : a;
+  const T* src = z.src;
+  T* dst = z.dst;
+  if (!first) {
+    b -= w_tiles;
+    const int t = b / a_tiles;
+    b -= t * a_tiles;
+    src += t * z.src_next;
+    dst += t * z.dst_next;
+  }
+  const int across = first ? w_across : a_across;
+  const int c0 = b % across * 32, r0 = b / across * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   for (int i = ty; i < 32; i += 8)
-    if (r0 + i < rows && c0 + tx < cols) tile[i][tx] = src[(int64_t)(r0 + i) * lds_ + c0 + tx];
+    if (r0 + i < z.rows && c0 + tx < z.cols) tile[i][tx] = src[(int64_t)(r0 + i) * z.lds + c0 + tx];
   __syncthreads();
   for (int i = ty; i < 32; i += 8)
-    if (c0 + i < cols && r0 + tx < rows) dst[(int64_t)(c0 + i) * ldd + r0 + tx] = tile[tx][i];
+    if (c0 + i < z.cols && r0 + tx < z.rows) dst[(int64_t)(c0 + i) * z.ldd + r0 + tx] = tile[tx][i];
 }
 
 // ---- host side --------------------------------------------------------------------------------------------
@@ -802,16 +839,22 @@ bool dtype_ok(int dtype) { return dtype == KGE_DT_F32 || dtype == KGE_DT_BF16; }
 bool ld_ok(int64_t ld, int64_t rows, int64_t cols) { return rows <= 1 || ld >= cols; }
 constexpr int64_t MAX_N = (int64_t)1 << 30, MAX_K = 1 << 20, MAX_R = 1024;
 constexpr int64_t FEW = 32;  // rows of the serving path
-#ifndef PSMALL
-#define PSMALL 2
-#endif
-constexpr int64_t PROJECT_SMALL = PSMALL;
+// 128-row tiles per CU below which tiles of 64 rows are taken (8192 x 512 x 512 with 237 adapters, one tile per CU:
+// 16.7 against 18.1 us; 1024 x 14541 x 512 with 64, 3.6 per CU: 52 against 47)
+constexpr int64_t PROJECT_SMALL = 2;
 int64_t rank_pad(int64_t r) { return (r + 15) / 16 * 16; }
 int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 template <typename F>
 int by_type(int dtype, F f) {
   return dtype == KGE_DT_F32 ? f((float*)nullptr) : f((__bf16*)nullptr);
+}
+// f(true or false as a type): whether all lengths are multiples of a fragment's elements
+template <typename T, typename F>
+int by_even(F f, std::initializer_list<int64_t> lengths) {
+  bool even = true;
+  for (int64_t l : lengths) even = even && l % Mma<T>::N == 0;
+  return even ? f(std::true_type{}) : f(std::false_type{});
 }
 #define KGE_TRY(expr)      \
   do {                     \
@@ -867,7 +910,7 @@ Save save_of(void* base, int64_t n, int64_t d, int64_t k, int64_t r) {
 
 struct BackWs {
   float* u;
-  void* wt;
+  void *wt, *at;
   int64_t ldwt;
   int64_t per;
   float *slabs_a, *slabs_b;
@@ -883,6 +926,8 @@ BackWs back_ws_of(void* base, int dtype, int64_t n, int64_t d, int64_t m, int64_
   s.ldwt = (m * es + 15) / 16 * 16 / es;
   s.wt = b + o;
   if (dx) o += round256(d * s.ldwt * es);
+  s.at = b + o;
+  if (dx) o += round256(k * r * d * es);
   s.per = grads_per(n, (da ? d : 0) + (db ? m : 0), r, es);
   s.slabs_a = (float*)(b + o);
   if (da) o += grads_ws(n, d, k, r, s.per);
@@ -903,9 +948,12 @@ int run_plan_h(const int64_t* ids, const T* x, int64_t ldx, int64_t n, int64_t d
                const float* scales, const Save& s, hipStream_t st) {
   const bool with_h = n * r * d * (int64_t)sizeof(T) <= 24 << 20;
   const int64_t groups = k + 2, blocks = groups + (with_h ? (n + 3) / 4 : 0);
-  plan_h_kernel<T><<<dim3((unsigned)blocks), dim3(PT), 0, st>>>(ids, (int)n, (int)k, s.perm, s.sid, s.start, (int)groups, x,
-                                                                ldx, (int)d, a, (int)r, (int)rank_pad(r), scales, s.h);
-  KGE_CHECK_LAUNCH();
+  KGE_TRY(by_even<T>([&](auto even) -> int {
+    plan_h_kernel<T, even.value><<<dim3((unsigned)blocks), dim3(PT), 0, st>>>(
+        ids, (int)n, (int)k, s.perm, s.sid, s.start, (int)groups, x, ldx, (int)d, a, (int)r, (int)rank_pad(r), scales, s.h);
+    KGE_CHECK_LAUNCH();
+    return 0;
+  }, {d}));
   return with_h || n == 0 ? 0 : run_shrink<T, true>(x, ldx, n, d, a, k, r, scales, s, s.h, st);
 }
 
@@ -914,9 +962,13 @@ int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int
                const Save& s, float* out, hipStream_t st) {
   const int rp = (int)rank_pad(r), splits = shrink_splits(n, cols, k, rp);
   const int64_t per_split = ((cols + splits - 1) / splits + 127) / 128 * 128;
-  shrink_kernel<T, BY_RANK><<<dim3((unsigned)(n / 16 + k), (unsigned)(rp / 16), (unsigned)splits), dim3(256), 0, st>>>(
-      v, ldv, (int)n, (int)cols, f, (int)k, (int)r, rp, scales, s.perm, s.start, (int)per_split, out);
-  KGE_CHECK_LAUNCH();
+  KGE_TRY(by_even<T>([&](auto even) -> int {
+    shrink_kernel<T, BY_RANK, even.value>
+        <<<dim3((unsigned)(n / 16 + k), (unsigned)(rp / 16), (unsigned)splits), dim3(256), 0, st>>>(
+            v, ldv, (int)n, (int)cols, f, (int)k, (int)r, rp, scales, s.perm, s.start, (int)per_split, out);
+    KGE_CHECK_LAUNCH();
+    return 0;
+  }, {cols}));
   if (splits == 1) return 0;
   const int64_t count = n * rp / 4;
   slabs_kernel<<<dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st>>>((f32x4*)out, count, splits);
@@ -924,7 +976,7 @@ int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int
   return 0;
 }
 
-template <typename T, bool BY_RANK, int BM>
+template <typename T, int BM>
 int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
                    int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
   // fp32 is bound by its matrix instructions: two workgroups per CU with two stages each keep them fed, and
@@ -933,20 +985,22 @@ int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, in
   const int64_t row_tiles = (n + BM - 1) / BM, tiles = row_tiles * ((m + BN - 1) / BN);
   KGE_REQUIRE(tiles < ((int64_t)1 << 31));
   const int yvec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T))) == 0 && ldy % 4 == 0;
-  project_kernel<T, BY_RANK, BM, STAGES><<<dim3((unsigned)tiles), dim3(256), 0, st>>>(
-      x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k, (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy, (int)row_tiles,
-      yvec);
-  KGE_CHECK_LAUNCH();
-  return 0;
+  return by_even<T>([&](auto even) -> int {
+    project_kernel<T, BM, STAGES, even.value><<<dim3((unsigned)tiles), dim3(256), 0, st>>>(
+        x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k, (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy,
+        (int)row_tiles, yvec);
+    KGE_CHECK_LAUNCH();
+    return 0;
+  }, {r});
 }
 
-template <typename T, bool BY_RANK>
+template <typename T>
 int run_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
                 int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
   const int64_t tiles = ((n + 127) / 128) * ((m + BN - 1) / BN);
   return tiles < PROJECT_SMALL * kge_num_cus()
-             ? launch_project<T, BY_RANK, 64>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st)
-             : launch_project<T, BY_RANK, 128>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st);
+             ? launch_project<T, 64>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st)
+             : launch_project<T, 128>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st);
 }
 
 template <typename T>
@@ -955,9 +1009,13 @@ int run_grads(Grad<T> g0, Grad<T> g1, int64_t n, int64_t k, int64_t r, const Sav
   g1.blocks = (int)((g1.cols * (int64_t)sizeof(T) + 255) / 256);
   const int64_t blocks = (int64_t)g0.blocks + g1.blocks, cols = (int64_t)g0.cols + g1.cols;
   KGE_REQUIRE(blocks <= 65535);
-  grads_kernel<T><<<dim3((unsigned)(n / per + k), (unsigned)blocks, (unsigned)(rank_pad(r) / 16)), dim3(256), 0, st>>>(
-      g0, g1, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per);
-  KGE_CHECK_LAUNCH();
+  KGE_TRY(by_even<T>([&](auto even) -> int {
+    grads_kernel<T, even.value>
+        <<<dim3((unsigned)(n / per + k), (unsigned)blocks, (unsigned)(rank_pad(r) / 16)), dim3(256), 0, st>>>(
+            g0, g1, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per);
+    KGE_CHECK_LAUNCH();
+    return 0;
+  }, {g0.cols, g1.cols}));
   if (n <= per) return 0;
   const int64_t join = std::max<int64_t>(1, std::min<int64_t>((r * cols + 255) / 256, 64));
   grads_join_kernel<T><<<dim3((unsigned)k, (unsigned)join), dim3(256), 0, st>>>(g0, g1, s.start, (int)per, (int)r);
@@ -970,30 +1028,34 @@ int run_few(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t l
             int64_t k, int64_t r, const int64_t* ids, const float* scales, float* h, T* y, int64_t ldy, hipStream_t st) {
   const int rp = (int)rank_pad(r);
   const dim3 grid((unsigned)((m + 15) / 16));
-  if (RB == 1 && n * r * d * (int64_t)sizeof(T) <= 32768 && n * rp * 4 <= 16384) {
-    project_few_kernel<T, 1, true><<<grid, dim3(256), (size_t)(n * rp * 4), st>>>(
-        x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r, rp, ids, scales, nullptr, y, ldy);
+  const bool here = RB == 1 && n * r * d * (int64_t)sizeof(T) <= 32768 && n * rp * 4 <= 16384;
+  return by_even<T>([&](auto even) -> int {
+    if (here) {
+      project_few_kernel<T, 1, true, even.value><<<grid, dim3(256), (size_t)(n * rp * 4), st>>>(
+          x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r, rp, ids, scales, nullptr, y, ldy);
+      KGE_CHECK_LAUNCH();
+      return 0;
+    }
+    h_few_kernel<T, even.value><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, a, (int)k, (int)r,
+                                                                                   rp, ids, scales, h);
+    KGE_CHECK_LAUNCH();
+    project_few_kernel<T, RB, false, even.value><<<grid, dim3(256), 0, st>>>(
+        x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r, rp, ids, scales, h, y, ldy);
     KGE_CHECK_LAUNCH();
     return 0;
-  }
-  h_few_kernel<T><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, a, (int)k, (int)r, rp, ids,
-                                                                       scales, h);
-  KGE_CHECK_LAUNCH();
-  project_few_kernel<T, RB, false><<<grid, dim3(256), 0, st>>>(x, ldx, (int)n, (int)d, w, ldw, (int)m, a, b, (int)k, (int)r,
-                                                               rp, ids, scales, h, y, ldy);
-  KGE_CHECK_LAUNCH();
-  return 0;
+  }, {d, r});
 }
 
+// W^T [d, ldwt] and every A_t^T [d, r]: dx is the projection of dy by them
 template <typename T>
-int run_transpose(const T* src, int64_t lds, int64_t rows, int64_t cols, T* dst, int64_t ldd, hipStream_t st) {
-  // the y dimension of a grid is limited: bands of rows
-  for (int64_t r0 = 0; r0 < rows; r0 += 65535 * (int64_t)32) {
-    const int64_t nr = std::min<int64_t>(rows - r0, 65535 * (int64_t)32);
-    transpose_kernel<T><<<dim3((unsigned)((cols + 31) / 32), (unsigned)((nr + 31) / 32)), dim3(256), 0, st>>>(
-        src + r0 * lds, lds, (int)nr, (int)cols, dst + r0, ldd);
-    KGE_CHECK_LAUNCH();
-  }
+int run_transpose(const T* w, int64_t ldw, int64_t m, int64_t d, const T* a, int64_t k, int64_t r, T* wt, int64_t ldwt, T* at,
+                  hipStream_t st) {
+  const int64_t across = (d + 31) / 32, w_tiles = across * ((m + 31) / 32), a_tiles = across * ((r + 31) / 32);
+  KGE_REQUIRE(w_tiles + a_tiles * k < (int64_t)1 << 31);
+  transpose_kernel<T><<<dim3((unsigned)(w_tiles + a_tiles * k)), dim3(256), 0, st>>>(
+      Flip<T>{w, ldw, 0, (int)m, (int)d, wt, ldwt, 0}, Flip<T>{a, d, r * d, (int)r, (int)d, at, r, r * d}, (int)w_tiles,
+      (int)across, (int)a_tiles, (int)across);
+  KGE_CHECK_LAUNCH();
   return 0;
 }
 
@@ -1023,7 +1085,7 @@ extern "C" int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_
     }
     KGE_TRY(run_plan_h<T>(ids, xt, ldx, n, d, at, k, r, scales, s, st));
     if (n == 0) return 0;
-    return run_project<T, false>(xt, ldx, n, d, wt, ldw, m, bt, k, r, s.h, s, yt, ldy, st);
+    return run_project<T>(xt, ldx, n, d, wt, ldw, m, bt, k, r, s.h, s, yt, ldy, st);
   });
 }
 
@@ -1049,8 +1111,8 @@ extern "C" int kge_adapter_backward(const void* dy, int dtype, int64_t lddy, int
     const T *dyt = (const T*)dy, *xt = (const T*)x, *wt = (const T*)w, *at = (const T*)a, *bt = (const T*)b;
     if (n > 0 && (dx || da)) KGE_TRY((run_shrink<T, false>(dyt, lddy, n, m, bt, k, r, scales, s, q.u, st)));
     if (n > 0 && dx) {
-      KGE_TRY(run_transpose<T>(wt, ldw, m, d, (T*)q.wt, q.ldwt, st));
-      KGE_TRY((run_project<T, true>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, at, k, r, q.u, s, (T*)dx, lddx, st)));
+      KGE_TRY(run_transpose<T>(wt, ldw, m, d, at, k, r, (T*)q.wt, q.ldwt, (T*)q.at, st));
+      KGE_TRY(run_project<T>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, (const T*)q.at, k, r, q.u, s, (T*)dx, lddx, st));
     }
     const Grad<T> ga{xt, ldx, (int)d, 0, q.u, (T*)da, 1, d, q.slabs_a}, gb{dyt, lddy, (int)m, 0, s.h, (T*)db, r, 1, q.slabs_b};
     const Grad<T> none{nullptr, 0, 0, 0, nullptr, nullptr, 0, 0, nullptr};

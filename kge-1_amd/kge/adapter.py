@@ -43,14 +43,17 @@ def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
 def _forward(x, w, a, b, ids, scales, for_backward):
     """(y, what the backward pass needs)"""
     n, d = x.shape
-    m, (k, r) = w.shape[0], a.shape[:2]
-    y = _padded(n, m, x)
-    size = L.lib().kge_adapter_save_size(n, d, k, r)
+    k, m, r = b.shape
+    per = 16 // x.element_size()
+    ld = (m + per - 1) // per * per  # rows of y start on 16 bytes
+    y = torch.empty(n, ld, device=x.device, dtype=x.dtype)
+    lib = L.lib()
+    size = lib.kge_adapter_save_size(n, d, k, r)
     save = torch.empty(size, device=x.device, dtype=torch.uint8)
-    L._check(L.lib().kge_adapter_forward(L.ptr(x), L.DTYPES[x.dtype], _ld(x), n, d, L.ptr(w), _ld(w), m, L.ptr(a), L.ptr(b),
-                                         k, r, L.ptr(ids), L.ptr(scales), L.ptr(y), _ld(y), L.ptr(save), size,
-                                         int(for_backward), L.stream()), "kge_adapter_forward")
-    return y, save
+    L._check(lib.kge_adapter_forward(x.data_ptr(), L.DTYPES[x.dtype], _ld(x), n, d, w.data_ptr(), _ld(w), m, a.data_ptr(),
+                                     b.data_ptr(), k, r, ids.data_ptr(), L.ptr(scales), y.data_ptr(), ld, save.data_ptr(),
+                                     size, for_backward, L.stream()), "kge_adapter_forward")
+    return y if ld == m else y[:, :m], save
 
 
 class _AdaptedProjection(torch.autograd.Function):
@@ -65,28 +68,47 @@ class _AdaptedProjection(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, a, b, scales, save = ctx.saved_tensors
         n, d = x.shape
-        m, (k, r) = w.shape[0], a.shape[:2]
-        want = [ctx.needs_input_grad[i] for i in (0, 2, 3)]
+        k, m, r = b.shape
+        want_x, _, want_a, want_b, _, _ = ctx.needs_input_grad
         with on_device_of(x):
             dy = _matrix(dy)
-            dx = _padded(n, d, x) if want[0] else None
-            da, db = (torch.empty_like(t) if w_ else None for t, w_ in zip((a, b), want[1:]))
-            size = L.lib().kge_adapter_backward_ws_size(L.DTYPES[x.dtype], n, d, m, k, r, *want)
+            dx = _padded(n, d, x) if want_x else None
+            da = torch.empty_like(a) if want_a else None
+            db = torch.empty_like(b) if want_b else None
+            lib, dtype = L.lib(), L.DTYPES[x.dtype]
+            size = lib.kge_adapter_backward_ws_size(dtype, n, d, m, k, r, want_x, want_a, want_b)
             ws = torch.empty(size, device=x.device, dtype=torch.uint8)
-            L._check(L.lib().kge_adapter_backward(
-                L.ptr(dy), L.DTYPES[dy.dtype], _ld(dy), n, m, L.ptr(x), _ld(x), d, L.ptr(w), _ld(w), L.ptr(a), L.ptr(b), k, r,
-                L.ptr(scales), L.ptr(save), save.numel(), L.ptr(dx), _ld(dx) if want[0] else d, L.ptr(da), L.ptr(db),
-                L.ptr(ws), size, L.stream()), "kge_adapter_backward")
+            L._check(lib.kge_adapter_backward(
+                dy.data_ptr(), dtype, _ld(dy), n, m, x.data_ptr(), _ld(x), d, w.data_ptr(), _ld(w), a.data_ptr(),
+                b.data_ptr(), k, r, L.ptr(scales), save.data_ptr(), save.numel(), L.ptr(dx), _ld(dx) if want_x else d,
+                L.ptr(da), L.ptr(db), ws.data_ptr(), size, L.stream()), "kge_adapter_backward")
         return dx, None, da, db, None, None
 
 
-def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
-                       scales: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y [n, m]: y_i = w x_i + scales[t] b[t] (a[t] x_i) for t = ids[i], y_i = w x_i for ids[i] = -1.
+def _as_they_are(x, w, a, b, ids, scales) -> bool:
+    """Whether the arguments are what the kernels take, with nothing to convert or to refuse (the usual case, seen
+    with few tensor accesses: a serving call is launch-bound); otherwise _checked says what is wrong."""
+    if L.CHECK_INDEX:
+        return False
+    dtype, dev, bs = x.dtype, x.get_device(), b.shape
+    if (dtype not in (torch.bfloat16, torch.float32) or w.dtype is not dtype or a.dtype is not dtype or b.dtype is not dtype
+            or len(bs) != 3 or w.get_device() != dev or a.get_device() != dev or b.get_device() != dev
+            or ids.get_device() != dev or ids.dtype is not torch.int64):
+        return False
+    k, m, r = bs
+    if len(a.shape) != 3 or len(x.shape) != 2:
+        return False
+    n, d = x.shape
+    if scales is not None and not (scales.dtype is torch.float32 and scales.shape == (k,) and scales.get_device() == dev
+                                   and scales.is_contiguous() and not scales.requires_grad):
+        return False
+    return (w.shape == (m, d) and a.shape == (k, r, d) and ids.shape == (n,) and min(d, m, k) >= 1 and 1 <= r <= MAX_RANK
+            and not w.requires_grad and x.is_contiguous() and w.is_contiguous() and a.is_contiguous() and b.is_contiguous()
+            and ids.is_contiguous())
 
-    x [n, d] requests in any order, w [m, d] shared and frozen (pass it detached), a [k, r, d] and
-    b [k, m, r] the adapters (ranks below r: padded with zeros), scales [k] (None: 1), all of one type, fp32
-    or bf16 (scales in any floating type, used in fp32).  Differentiable in x, a and b."""
+
+def _checked(x, w, a, b, ids, scales):
+    """The arguments as the kernels take them, or an error that says what is wrong."""
     if x.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"x: expected float32 or bfloat16, got {x.dtype}")
     dtype, dev = x.dtype, x.get_device()  # (-1: CPU)
@@ -119,8 +141,19 @@ def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: tor
         lo, hi = int(ids.min()), int(ids.max())
         if lo < -1 or hi >= k:
             raise IndexError(f"adapter id: out of range [{lo}, {hi}] for {k} adapters (-1: none)")
+    return _matrix(x), _matrix(w), a.contiguous(), b.contiguous(), ids, scales
+
+
+def adapted_projection(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
+                       scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y [n, m]: y_i = w x_i + scales[t] b[t] (a[t] x_i) for t = ids[i], y_i = w x_i for ids[i] = -1.
+
+    x [n, d] requests in any order, w [m, d] shared and frozen (pass it detached), a [k, r, d] and
+    b [k, m, r] the adapters (ranks below r: padded with zeros), scales [k] (None: 1), all of one type, fp32
+    or bf16 (scales in any floating type, used in fp32).  Differentiable in x, a and b."""
+    if not _as_they_are(x, w, a, b, ids, scales):
+        x, w, a, b, ids, scales = _checked(x, w, a, b, ids, scales)
     L.require_device(x)
-    x, w, a, b = _matrix(x), _matrix(w), a.contiguous(), b.contiguous()
     with on_device_of(x):
         if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
             return _AdaptedProjection.apply(x, w, a, b, ids, scales)
