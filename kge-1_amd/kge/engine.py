@@ -546,6 +546,28 @@ def score_all(kind: int, direction: int, precision: int, l_norm: float, ent: tor
                            L.idx64(ridx), tab, L.idx64(tidx))
 
 
+def score_all_adapted(kind: int, direction: int, ent: torch.Tensor, eidx: torch.Tensor, rel: torch.Tensor,
+                      ridx: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
+                      scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """score_all of the frozen fp32 tables against every row of ent, row i with the low-rank adapter ids[i]
+    (-1: none) between its query and the candidates: q_i T^T + scales[t] (q_i a[t]^T) b[t]^T.  a [k, r, query
+    width] and b [k, E, r] are fp32; gradients flow into them only.  Bilinear models (a distance is not a
+    projection of the query)."""
+    if kind not in BILINEAR:
+        raise ValueError("low-rank adapters stand beside a dot product of query and candidate: bilinear models only")
+    for t, what in ((ent, "ent"), (rel, "rel")):
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: the tables are frozen beside adapters, pass them detached")
+    n = eidx.numel()
+    if ridx.numel() != n:
+        raise ValueError(f"{n} entities, {ridx.numel()} relations: expected one each per query")
+    L.require_device(ent, rel)
+    with on_device_of(ent):
+        q = (L.prep_query(kind, direction, ent, eidx, rel, ridx, n, ent.shape[1], rel.shape[1]) if n
+             else ent.new_empty(0, L.query_width(kind, ent.shape[1])))
+    return adapted_projection(q, window(kind, direction, ent), a, b, ids, scales)
+
+
 class _NoGradCtx:
     """Stands in for an autograd context where no gradient is taken."""
     needs_input_grad = (False,) * 16
@@ -826,4 +848,4 @@ def score_spo_emb(kind: int, l_norm: float, s_emb, p_emb, o_emb) -> torch.Tensor
 # Post-training operators: losses on sampled or preferred answers
 from .label_losses import (label_logprobs, policy_loss, policy_loss_grad, preference_loss,  # noqa: E402, F401
                            preference_loss_grad)
-from .adapter import adapted_projection  # noqa: E402, F401  (low-rank adapters beside a shared projection)
+from .adapter import adapted_projection, on_device_of  # noqa: E402, F401  (low-rank adapters beside a shared projection)

@@ -146,6 +146,16 @@ class RelationalScorer(KgeBase):
         return engine.score_all(self.engine_kind, d, self.precision(), self.l_norm(), ent, e_idx, rel, p_idx,
                                 ent, cand_idx)
 
+    def score_lookup_adapted(self, ent: Tensor, rel: Tensor, e_idx: Tensor, p_idx: Tensor, direction: str, adapters,
+                             ids: Tensor) -> Tensor:
+        """score_lookup of the frozen tables against all entities, row i with adapter ids[i] of ``adapters``
+        (kge/adapter.py; -1: none).  Gradients flow into the adapters only."""
+        from .. import engine, _lib
+
+        d = _lib.DIR_SP if direction == "sp_" else _lib.DIR_PO
+        return engine.score_all_adapted(self.engine_kind, d, ent.detach(), e_idx, rel.detach(), p_idx, adapters.a,
+                                        adapters.b, ids, adapters.scales)
+
     def score_lookup_parts(self, ent: Tensor, rel: Tensor, parts, cand_idx: Optional[Tensor] = None,
                            want_q: bool = False, out: Optional[Tensor] = None):
         """Several query batches (direction "sp_" / "_po", e_idx, p_idx) against the same
@@ -430,6 +440,37 @@ class KgeModel(KgeBase):
         o = self.get_o_embedder().embed(o)
         p = self.get_p_embedder().embed(p)
         return self._scorer.score_emb(s, p, o, combine="_po")
+
+    # --- a trained model with small corrections of its own per client, domain or relation
+    def create_adapters(self, num_adapters: int, rank: int, alpha: Optional[float] = None):
+        """``num_adapters`` low-rank adapters (kge/adapter.py) of this model's width, on its device; new ones
+        change nothing.  They are parameters of their own: the model's tables stay as they are."""
+        from ..adapter import LowRankAdapters
+        from .. import _lib
+
+        ent, _ = self._tables_for_adapters()
+        return LowRankAdapters(num_adapters, rank, _lib.query_width(self._scorer.engine_kind, ent.shape[1]),
+                               ent.shape[0], alpha, device=ent.device)
+
+    def score_sp_adapted(self, s: Tensor, p: Tensor, adapters, ids: Tensor) -> Tensor:
+        """[n, E] score_sp(s, p), row i corrected by adapter ids[i] (-1: none; one batch may mix them all).
+        Differentiable in the adapters; the model is frozen.  fp32."""
+        ent, rel = self._tables_for_adapters()
+        return self._scorer.score_lookup_adapted(ent, rel, s, p, "sp_", adapters, ids)
+
+    def score_po_adapted(self, p: Tensor, o: Tensor, adapters, ids: Tensor) -> Tensor:
+        """[n, E] score_po(p, o) with adapters (see score_sp_adapted)."""
+        ent, rel = self._tables_for_adapters()
+        return self._scorer.score_lookup_adapted(ent, rel, o, p, "_po", adapters, ids)
+
+    def _tables_for_adapters(self):
+        from .. import engine
+
+        tabs = self._lookup_tables()
+        if tabs is None or self._scorer.engine_kind not in engine.BILINEAR:
+            raise ValueError(f"adapters: {self.model} needs plain lookup embedders (no dropout in training mode) and a "
+                             "bilinear scorer")
+        return tabs
 
     def score_sp_xent(self, s: Tensor, p: Tensor, o: Tensor, scale: float) -> Optional[Tensor]:
         """scale * sum_i CrossEntropy(score_sp(s, p)[i, :], o[i]) fused into the engine, or

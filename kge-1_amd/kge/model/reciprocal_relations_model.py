@@ -46,6 +46,11 @@ class ReciprocalRelationsModel(KgeModel):
         o = self.get_o_embedder().embed(o)
         return self._scorer.score_emb(o, p, s, combine="sp_")
 
+    def score_po_adapted(self, p: Tensor, o: Tensor, adapters, ids: Tensor) -> Tensor:
+        """(?, p, o) is scored as (o, p + R, ?) (reciprocal_relations_model.py:67-74)."""
+        ent, rel = self._tables_for_adapters()
+        return self._scorer.score_lookup_adapted(ent, rel, o, p + self.dataset.num_relations(), "sp_", adapters, ids)
+
     def _xent_dropout_po(self, p, o, labels, scale, l_ptr=None, smoothing=0.0):
         """The fused loss of (?, p, o) queries with dropout in the embedders: dropped rows drawn
         in score_po's order (reciprocal_relations_model.py:67-74: all subjects, p + R, then o),
