@@ -729,9 +729,12 @@ Ws ws_of(void* base, int64_t n, int64_t m, int dtype, int64_t pairs) {
   return w;
 }
 
+bool temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }  // (1 / t is a 32-bit factor, neither 0 nor infinite)
+
+// (a launch has at most n + FILL workgroups)
 bool shape_ok(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels) {
   return dtype >= KGE_DT_F32 && dtype <= KGE_DT_F16 && n >= 0 && m >= 1 && m < (int64_t)1 << 31 && lds >= (n > 1 ? m : 0) &&
-         n <= ((int64_t)1 << 31) / (FILL + 1) && (n == 0 || (s && labels)) &&
+         n <= (int64_t)1 << 30 && (n == 0 || (s && labels)) &&
          (reinterpret_cast<uintptr_t>(s) % elem_size(dtype)) == 0;
 }
 
@@ -824,7 +827,7 @@ extern "C" int64_t kge_label_ws_size(int64_t n, int64_t m, int dtype, int64_t pa
 extern "C" int kge_label_logprobs(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
                                   double temperature, float* logp, float* stats, void* ws, int64_t ws_bytes,
                                   void* stream) {
-  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature > 0.0);
+  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature_ok(temperature));
   if (n == 0) return 0;
   const Ws w = ws_of(ws, n, m, dtype, 0);
   KGE_REQUIRE(logp && ws && ws_bytes >= w.bytes && aligned16(ws));
@@ -839,7 +842,7 @@ extern "C" int kge_label_logprobs(const void* s, int dtype, int64_t lds, int64_t
 extern "C" int kge_label_grad(const void* s, int dtype, int64_t lds, int64_t n, int64_t m, const int64_t* labels,
                               double temperature, const float* stats, const float* coef, const float* gscale, void* g,
                               int64_t ldg, void* stream) {
-  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature > 0.0);
+  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature_ok(temperature));
   if (n == 0) return 0;
   KGE_REQUIRE(stats && coef && g && ldg >= (n > 1 ? m : 0) && (reinterpret_cast<uintptr_t>(g) % elem_size(dtype)) == 0);
   const Temp t = temp_of(temperature);
@@ -855,7 +858,7 @@ extern "C" int kge_policy_loss(const void* s, int dtype, int64_t lds, int64_t n,
                                const float* weights, double clip_low, double clip_high, double kl, double temperature,
                                double scale, float* loss, float* logp, float* stats, float* coef, void* g, int64_t ldg,
                                void* ws, int64_t ws_bytes, void* stream) {
-  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature > 0.0 && loss);
+  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature_ok(temperature) && loss);
   const hipStream_t st = as_stream(stream);
   if (n == 0) return run_total(nullptr, 0, loss, st);
   const Ws w = ws_of(ws, n, m, dtype, 0);
@@ -887,7 +890,7 @@ extern "C" int kge_preference_loss(const void* s, int dtype, int64_t lds, int64_
                                    double smoothing, int average, double temperature, double scale, float* loss,
                                    float* seq_logp, float* logp, float* stats, float* coef, void* g, int64_t ldg,
                                    void* ws, int64_t ws_bytes, void* stream) {
-  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature > 0.0 && loss && pairs >= 0);
+  KGE_REQUIRE(shape_ok(s, dtype, lds, n, m, labels) && temperature_ok(temperature) && loss && pairs >= 0);
   const hipStream_t st = as_stream(stream);
   const Ws w = ws_of(ws, n, m, dtype, pairs);
   KGE_REQUIRE((n == 0 && pairs == 0) || (ws && ws_bytes >= w.bytes && aligned16(ws)));

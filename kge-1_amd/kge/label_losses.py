@@ -101,8 +101,8 @@ def _vector(t: Optional[torch.Tensor], n: int, scores: torch.Tensor, what: str) 
 
 def _temperature(temperature: float) -> float:
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature={temperature}: expected a positive number")
+    if not 1e-30 <= temperature <= 1e30:  # log2(e) / temperature is a 32-bit factor, neither 0 nor infinite
+        raise ValueError(f"temperature={temperature}: expected a number in [1e-30, 1e30]")
     return temperature
 
 
@@ -127,8 +127,7 @@ def _grad_buffer(scores: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Ten
         if ld > m + 64:
             per = 16 // scores.element_size()
             ld = (m + per - 1) // per * per
-        buf = torch.empty(n, ld, device=scores.device, dtype=scores.dtype)
-        return buf if ld == m else buf[:, :m]
+        return torch.empty_strided((n, m), (ld, 1), device=scores.device, dtype=scores.dtype)
     if out.shape != scores.shape or out.dtype != scores.dtype or out.device != scores.device:
         raise ValueError("out: expected the scores' shape, type and device")
     if (m > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < m):
@@ -140,6 +139,8 @@ def _grad_buffer(scores: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Ten
         es, a, b = out.element_size(), out.data_ptr(), scores.data_ptr()
         if a < b + ((n - 1) * _ld(scores) + m) * es and b < a + ((n - 1) * _ld(out) + m) * es:
             raise ValueError("out: overlaps the scores without being the same rows")
+    if not out.is_inference():  # a graph that has saved the scores sees that they are gone
+        torch.autograd.graph.increment_version(out)
     return out
 
 
@@ -288,7 +289,7 @@ class _Preference:
         self.smoothing, self.average = _finite(smoothing, "smoothing", 0.0, 1.0), bool(average)
         self.scores = _score_rows(scores)
         self.labels = _labels(labels, self.scores)
-        if seq_ptr.dim() != 1 or seq_ptr.numel() % 2 != 1 or seq_ptr.is_floating_point():
+        if seq_ptr.dim() != 1 or seq_ptr.numel() % 2 != 1 or seq_ptr.is_floating_point() or seq_ptr.dtype == torch.bool:
             raise ValueError("seq_ptr: expected 2 pairs + 1 ascending row numbers (two sequences per pair), got "
                              f"{list(seq_ptr.shape)} {seq_ptr.dtype}")
         _same_device(seq_ptr, self.scores, "seq_ptr")

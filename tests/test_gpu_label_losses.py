@@ -466,3 +466,44 @@ def test_rows_past_32_bit_offsets(engine):
     want = -(onehot - p)
     assert ((src.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2 * E[:, None] + 1e-30).all()
     assert float(grad[2].float().abs().max()) == 0.0
+
+
+def test_more_than_a_million_short_rows(engine):
+    n, m = 1_100_003, 5
+    s, y = block(n, m, torch.float32, 11, masked=False)
+    leaf = s.detach().requires_grad_(True)
+    logp = engine.label_logprobs(leaf, y)
+    (g,) = torch.autograd.grad(logp.sum(), leaf)
+    l, p, e, E = formulas(s, y, 1.0)
+    check_logp(logp, l, E, y)
+    check_grad(g, s, y, 1.0, torch.ones(n).double(), torch.zeros(n).double(), p, e, E)
+    loss, _ = engine.policy_loss(s, y, torch.ones(n, device="cuda"), logp.detach(), scale=1 / n)
+    # r = exp(l - old) with old = l rounded: 1 to U |l|; minus the share of labelled rows, rounded
+    assert abs(float(loss) + float((y >= 0).double().mean())) <= 1.01 * U * float(l.abs().max()) + 2 * U
+
+
+def test_a_gradient_written_over_saved_scores_is_noticed(engine):
+    s, y = block(6, 40, torch.float32, 4, masked=False)
+    v = torch.ones(6, device="cuda")
+    leaf = s.detach().requires_grad_(True)
+    scores = leaf * 1.0
+    logp = engine.label_logprobs(scores, y)  # its backward pass reads the scores
+    engine.policy_loss_grad(scores, y, v, v, out=scores.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        logp.sum().backward()
+    with torch.inference_mode():  # no graph to protect
+        t = s.clone()
+        engine.policy_loss_grad(t, y, v, v, out=t)
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e30])
+def test_the_largest_and_smallest_temperatures(engine, temperature):
+    s, y = block(4, 40, torch.float32, 4, masked=True)
+    logp = engine.label_logprobs(s, y, temperature)
+    assert not torch.isnan(logp).any()
+    if temperature > 1:  # uniform over the finite scores; |s| / 1e30 is below every rounding
+        ref = torch.where(y.cpu() >= 0, -torch.isfinite(s.cpu()).sum(1).double().log(), 0.0)
+        assert ((logp.cpu().double() - ref).abs() <= 44 * U + 2 * U * ref.abs()).all()
+    else:  # the largest score alone
+        best = s.gather(1, y.clamp(min=0)[:, None])[:, 0] == s.max(1).values
+        assert ((logp == 0) == (best | (y < 0))).all()

@@ -116,3 +116,18 @@ def test_workspace_covers_parts_rows_and_losses(n, m, pairs):
         size = L.lib().kge_label_ws_size(n, m, code, pairs)
         least = n * 8 + n * 4 + max(n, pairs) * 8
         assert least + parts * 8 <= size <= least + (n + 2048) * 8 + 4 * 256
+
+
+@pytest.mark.parametrize("temperature", [1e-31, 1e31])
+def test_temperatures_whose_factor_is_no_32_bit_number_are_refused(temperature):
+    """log2(e) / temperature would be infinite (0 * inf is NaN for a row's largest score) or 0 (-inf * 0)."""
+    s, y = _block()
+    with pytest.raises(ValueError, match="temperature"):
+        engine.label_logprobs(s, y, temperature)
+    assert L.lib().kge_label_logprobs(None, 0, 5, 0, 5, None, temperature, None, None, None, 0, None) == 1001
+
+
+def test_seq_ptr_of_booleans_refused():
+    s, y = _block()
+    with pytest.raises(ValueError, match="seq_ptr"):
+        engine.preference_loss(s, y, torch.tensor([False, True, True]))
