@@ -185,6 +185,110 @@ __device__ __forceinline__ void plan_group(int g, const int64_t* __restrict__ id
   }
 }
 
+// ---- plan of many rows: a stable radix sort by group --------------------------------------------------------
+// The plan above reads every id once per group.  Beyond SORT_FROM reads the order comes from one pass (two from 2048
+// groups on) over digits of 11 bits: each wave counts the digits of its own rows (sort_count), the counts of a digit
+// are summed over the waves in order (sort_scan), and each wave puts its rows where the sums say, equal digits within
+// 64 rows in row order by ballots (sort_put): no global atomics, the same order as above.
+constexpr int DIGIT = 11, BINS = 1 << DIGIT;
+
+__device__ __forceinline__ int group_of(int64_t v, int k) { return v == -1 ? k : (v < 0 || v >= k ? k + 1 : (int)v); }
+
+__global__ void __launch_bounds__(64) sort_count_kernel(const int64_t* __restrict__ ids, int n, int k, const int* __restrict__ src,
+                                                        int shift, int bins, int rows, int* __restrict__ counts) {
+  __shared__ int count[BINS];
+  const int lane = threadIdx.x;
+  const int64_t lo = (int64_t)blockIdx.x * rows, hi = lo + rows < n ? lo + rows : n;
+  for (int b = lane; b < bins; b += 64) count[b] = 0;
+  __syncthreads();
+  for (int64_t i = lo + lane; i < hi; i += 64)
+    atomicAdd(&count[(group_of(ids[src ? src[i] : i], k) >> shift) & (BINS - 1)], 1);  // (in LDS; a count has no order)
+  __syncthreads();
+  for (int b = lane; b < bins; b += 64) counts[(int64_t)b * gridDim.x + blockIdx.x] = count[b];
+}
+
+// exclusive sum over a wave; total in every lane
+__device__ __forceinline__ int wave_before(int v, int lane, int& total) {
+  int x = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off, 64);
+    x += lane >= off ? y : 0;
+  }
+  total = __shfl(x, 63, 64);
+  return x - v;
+}
+
+// one wave per digit
+__global__ void __launch_bounds__(64) sort_scan_kernel(int* __restrict__ counts, int blocks, int* __restrict__ totals) {
+  const int lane = threadIdx.x;
+  int* c = counts + (int64_t)blockIdx.x * blocks;
+  int before = 0;
+  for (int b0 = 0; b0 < blocks; b0 += 64) {
+    const int v = b0 + lane < blocks ? c[b0 + lane] : 0;
+    int total;
+    const int x = wave_before(v, lane, total);
+    if (b0 + lane < blocks) c[b0 + lane] = before + x;
+    before += total;
+  }
+  if (lane == 0) totals[blockIdx.x] = before;
+}
+
+// sid: written by the last pass
+__global__ void __launch_bounds__(64) sort_put_kernel(const int64_t* __restrict__ ids, int n, int k, const int* __restrict__ src,
+                                                      int shift, int bins, int rows, const int* __restrict__ counts,
+                                                      const int* __restrict__ totals, int* __restrict__ dst,
+                                                      int* __restrict__ sid) {
+  __shared__ int next[BINS];
+  const int lane = threadIdx.x;
+  const int64_t lo = (int64_t)blockIdx.x * rows, hi = lo + rows < n ? lo + rows : n;
+  int before = 0;
+  for (int b0 = 0; b0 < bins; b0 += 64) {
+    const int b = b0 + lane;
+    int total;
+    const int x = wave_before(b < bins ? totals[b] : 0, lane, total);
+    if (b < bins) next[b] = before + x + counts[(int64_t)b * gridDim.x + blockIdx.x];
+    before += total;
+  }
+  __syncthreads();
+  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+    const bool in = i0 + lane < hi;
+    const int row = in ? (src ? src[i0 + lane] : (int)(i0 + lane)) : 0;
+    const int g = in ? group_of(ids[row], k) : 0, digit = (g >> shift) & (BINS - 1);
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < DIGIT; ++b) {
+      const bool one = (digit >> b) & 1;
+      const uint64_t ones = __ballot(one);
+      same &= one ? ones : ~ones;
+    }
+    const uint64_t below = same & ((1ull << lane) - 1);
+    const int to = next[digit] + __popcll(below);
+    __syncthreads();  // every lane has read
+    if (in && below == 0) next[digit] += __popcll(same);
+    __syncthreads();
+    if (in) {
+      dst[to] = row;
+      if (sid) sid[to] = g;
+    }
+  }
+}
+
+// start[g]: the first place whose group is g or above
+__global__ void __launch_bounds__(256) sort_start_kernel(const int* __restrict__ sid, int n, int groups, int* __restrict__ start) {
+  const int g = blockIdx.x * 256 + threadIdx.x;
+  if (g > groups) return;
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (sid[mid] < g)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  start[g] = lo;
+}
+
 // ---- h of one row, 16 ranks, columns [c_lo, c_hi), by one wave ------------------------------------------------
 // The matrix instruction with the same row in all 16 places does the sums; put(q, value) for q < 16 (0 from r on).
 // at: the ranks' rows of A_t, ld apart.
@@ -348,7 +452,7 @@ __device__ __forceinline__ u32x4 h_frag<__bf16>(const float* h, int q0, int fs) 
   for (int e = 0; e < 8; ++e) {
     __bf16 hi, lo;
     split_bf16(p[e], hi, lo);
-    o[e] = fs & 2 ? lo : hi;
+    o[e] = fs & 2 ? (isfinite(p[e] - (float)hi) ? lo : (__bf16)0.f) : hi;  // (an infinity has no rest)
   }
   return __builtin_bit_cast(u32x4, o);
 }
@@ -706,21 +810,26 @@ struct Grad {
 };
 constexpr int GU = 4;
 
+// An adapter of more than `per` rows from `row0` on has the slabs first_slab .. + chunks - 1: distinct, as chunks <=
+// floor(2 rows / per) there, and below 2 n / per + 1.
+__device__ __forceinline__ int64_t first_slab(int row0, int per) { return 2 * (int64_t)row0 / per; }
+
 template <typename T, bool EVEN>
 __global__ void __launch_bounds__(256) grads_kernel(Grad<T> g0, Grad<T> g1, int rp, int k, int r,
                                                     const int* __restrict__ perm, const int* __restrict__ start, int per) {
   constexpr int N = Mma<T>::N;
   typedef T vec __attribute__((ext_vector_type(N)));
   __shared__ f32x4 part[4][N][64];
-  const Chunk ch = chunk_of(blockIdx.x, start, k, per);
+  const int blocks = g0.blocks + g1.blocks, slot = blockIdx.x / blocks, by = blockIdx.x - slot * blocks;
+  const Chunk ch = chunk_of(slot, start, k, per);
   if (ch.c < 0 || ch.c >= ch.chunks) return;
-  const bool second = (int)blockIdx.y >= g0.blocks;
+  const bool second = by >= g0.blocks;
   const T* __restrict__ v = second ? g1.v : g0.v;
   const float* __restrict__ h = second ? g1.h : g0.h;
   const int64_t ldv = second ? g1.ldv : g0.ldv;
-  const int cols = second ? g1.cols : g0.cols, block = second ? blockIdx.y - g0.blocks : blockIdx.y;
+  const int cols = second ? g1.cols : g0.cols, block = second ? by - g0.blocks : by;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fs = lane >> 4;
-  const int c0 = block * 16 * N + fr * N, q0 = blockIdx.z * 16;
+  const int c0 = block * 16 * N + fr * N, q0 = blockIdx.y * 16;
   f32x4 acc[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -756,7 +865,7 @@ __global__ void __launch_bounds__(256) grads_kernel(Grad<T> g0, Grad<T> g1, int 
     sum[j] = (part[0][z][lane] + part[1][z][lane]) + (part[2][z][lane] + part[3][z][lane]);
   }
   if (ch.chunks > 1) {
-    float* sl = (second ? g1.slabs : g0.slabs) + (int64_t)blockIdx.x * r * cols;  // [r][cols]
+    float* sl = (second ? g1.slabs : g0.slabs) + (first_slab(ch.row0 - ch.c * per, per) + ch.c) * r * cols;  // [r][cols]
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -789,14 +898,14 @@ __global__ void __launch_bounds__(256) grads_join_kernel(Grad<T> g0, Grad<T> g1,
   const int t = blockIdx.x;
   const int s0 = start[t], chunks = (start[t + 1] - s0 + per - 1) / per;
   if (chunks <= 1) return;
-  const int64_t slot = s0 / per + t;
+  const int64_t slab = first_slab(s0, per);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const Grad<T>& g = w ? g1 : g0;
     const int64_t size = (int64_t)r * g.cols;
     for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.y * 256) {
       float a = 0.f;
-      for (int c = 0; c < chunks; ++c) a += g.slabs[(slot + c) * size + i];
+      for (int c = 0; c < chunks; ++c) a += g.slabs[(slab + c) * size + i];
       const int64_t q = i / g.cols, col = i - q * g.cols;
       g.out[t * size + col * g.oc + q * g.oq] = (T)a;
     }
@@ -813,7 +922,8 @@ struct Flip {
   int64_t ldd, dst_next;
 };
 template <typename T>
-__global__ void __launch_bounds__(256) transpose_kernel(Flip<T> w, Flip<T> a, int w_tiles, int w_across, int a_tiles, int a_across) {
+__global__ void __launch_bounds__(256) transpose_kernel(Flip<T> w, Flip<T> a, int w_tiles, int w_across, int a_tiles, int a_across,
+                                                        const int* __restrict__ start) {
   __shared__ T tile[32][33];
   int b = blockIdx.x;
   const bool first = b < w_tiles;
@@ -824,6 +934,7 @@ __global__ void __launch_bounds__(256) transpose_kernel(Flip<T> w, Flip<T> a, in
     b -= w_tiles;
     const int t = b / a_tiles;
     b -= t * a_tiles;
+    if (start[t] == start[t + 1]) return;  // no row has this adapter (the whole workgroup)
     src += t * z.src_next;
     dst += t * z.dst_next;
   }
@@ -886,14 +997,25 @@ int64_t grads_per(int64_t n, int64_t cols, int64_t r, int es) {
   const int64_t chunks = std::max<int64_t>(1, 2048 / blocks);
   return std::max<int64_t>(1024, ((n + chunks - 1) / chunks + 63) / 64 * 64);
 }
-int64_t grads_ws(int64_t n, int64_t cols, int64_t k, int64_t r, int64_t per) {
-  return n <= per ? 0 : round256((n / per + k) * r * cols * 4);
+int64_t grads_ws(int64_t n, int64_t cols, int64_t r, int64_t per) {
+  return n <= per ? 0 : round256((2 * n / per + 1) * r * cols * 4);
 }
+
+// Whether the plan is sorted: by the id reads of the other one, whose fewest rows cost as much as 1024 (a workgroup's
+// step) and fewest groups as 512 (they run at once)
+// (65536 rows of 237 adapters 46 us against 36 sorted, 2^20 rows 576 against 141, 8192 rows of 16000 adapters 142 against
+// 43; below: 32768 rows of 237 27 against 29 and three launches more, 8192 rows of 2000 32 against 54)
+constexpr int64_t SORT_FROM = 3 << 23;
+bool plan_sorted(int64_t n, int64_t k) { return std::max<int64_t>(n, 1024) * std::max<int64_t>(k + 2, 512) > SORT_FROM; }
+// rows of a wave: 512, or what leaves about 1024 waves
+int64_t sort_rows(int64_t n) { return std::max<int64_t>(512, (n + 1023) / 1024); }
+int64_t sort_bins(int64_t k) { return std::min<int64_t>(k + 2, BINS); }
 
 // what the forward pass leaves for the backward one: the plan and h
 struct Save {
   int *perm, *sid, *start;
   float* h;
+  int *order, *counts, *totals;  // the sort's
   int64_t bytes;
 };
 Save save_of(void* base, int64_t n, int64_t d, int64_t k, int64_t r) {
@@ -908,6 +1030,12 @@ Save save_of(void* base, int64_t n, int64_t d, int64_t k, int64_t r) {
   o += round256((k + 3) * 4);
   s.h = (float*)(b + o);
   o += round256(n * rank_pad(r) * shrink_splits(n, d, k, rank_pad(r)) * 4);
+  s.order = (int*)(b + o);
+  if (plan_sorted(n, k)) o += round256(n * 4);
+  s.counts = (int*)(b + o);
+  if (plan_sorted(n, k)) o += round256(((n + sort_rows(n) - 1) / sort_rows(n)) * sort_bins(k) * 4);
+  s.totals = (int*)(b + o);
+  if (plan_sorted(n, k)) o += round256(sort_bins(k) * 4);
   s.bytes = o;
   return s;
 }
@@ -934,15 +1062,35 @@ BackWs back_ws_of(void* base, int dtype, int64_t n, int64_t d, int64_t m, int64_
   if (dx) o += round256(k * r * d * es);
   s.per = grads_per(n, (da ? d : 0) + (db ? m : 0), r, es);
   s.slabs_a = (float*)(b + o);
-  if (da) o += grads_ws(n, d, k, r, s.per);
+  if (da) o += grads_ws(n, d, r, s.per);
   s.slabs_b = (float*)(b + o);
-  if (db) o += grads_ws(n, m, k, r, s.per);
+  if (db) o += grads_ws(n, m, r, s.per);
   s.bytes = o;
   return s;
 }
 
+int run_sort(const int64_t* ids, int64_t n, int64_t k, const Save& s, hipStream_t st) {
+  const int rows = (int)sort_rows(n), blocks = (int)((n + rows - 1) / rows), groups = (int)k + 2;
+  for (int shift = 0; shift == 0 || groups > 1 << shift; shift += DIGIT) {
+    const bool last = groups <= 1 << (shift + DIGIT);
+    const int* src = shift == 0 ? nullptr : s.order;
+    const int bins = std::min(BINS, ((groups - 1) >> shift) + 1);
+    sort_count_kernel<<<dim3(blocks), dim3(64), 0, st>>>(ids, (int)n, (int)k, src, shift, bins, rows, s.counts);
+    KGE_CHECK_LAUNCH();
+    sort_scan_kernel<<<dim3(bins), dim3(64), 0, st>>>(s.counts, blocks, s.totals);
+    KGE_CHECK_LAUNCH();
+    sort_put_kernel<<<dim3(blocks), dim3(64), 0, st>>>(ids, (int)n, (int)k, src, shift, bins, rows, s.counts, s.totals,
+                                                      last ? s.perm : s.order, last ? s.sid : nullptr);
+    KGE_CHECK_LAUNCH();
+  }
+  sort_start_kernel<<<dim3((unsigned)(groups / 256 + 1)), dim3(256), 0, st>>>(s.sid, (int)n, groups, s.start);
+  KGE_CHECK_LAUNCH();
+  return 0;
+}
+
 // The plan, and h of every row: in the same launch where each row reading its own A_t costs little (24 MiB from
-// the L2s), else by adapter afterwards.
+// the L2s, 2048 rows: 8192 rows of 16 columns take 14.1 us, 10.5 by adapter) or hardly two share one, else by adapter
+// afterwards.
 template <typename T, bool BY_RANK>
 int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int64_t k, int64_t r, const float* scales,
                const Save& s, float* out, hipStream_t st);
@@ -950,14 +1098,16 @@ int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int
 template <typename T>
 int run_plan_h(const int64_t* ids, const T* x, int64_t ldx, int64_t n, int64_t d, const T* a, int64_t k, int64_t r,
                const float* scales, const Save& s, hipStream_t st) {
-  const bool with_h = n * r * d * (int64_t)sizeof(T) <= 24 << 20;
-  const int64_t groups = k + 2, blocks = groups + (with_h ? (n + 3) / 4 : 0);
-  KGE_TRY(by_even<T>([&](auto even) -> int {
-    plan_h_kernel<T, even.value><<<dim3((unsigned)blocks), dim3(PT), 0, st>>>(
-        ids, (int)n, (int)k, s.perm, s.sid, s.start, (int)groups, x, ldx, (int)d, a, (int)r, (int)rank_pad(r), scales, s.h);
-    KGE_CHECK_LAUNCH();
-    return 0;
-  }, {d}));
+  const bool with_h = (n <= 2048 && n * r * d * (int64_t)sizeof(T) <= 24 << 20) || k >= n, sorted = plan_sorted(n, k);
+  const int64_t groups = sorted ? 0 : k + 2, blocks = groups + (with_h ? (n + 3) / 4 : 0);
+  if (sorted) KGE_TRY(run_sort(ids, n, k, s, st));
+  if (blocks > 0)
+    KGE_TRY(by_even<T>([&](auto even) -> int {
+      plan_h_kernel<T, even.value><<<dim3((unsigned)blocks), dim3(PT), 0, st>>>(
+          ids, (int)n, (int)k, s.perm, s.sid, s.start, (int)groups, x, ldx, (int)d, a, (int)r, (int)rank_pad(r), scales, s.h);
+      KGE_CHECK_LAUNCH();
+      return 0;
+    }, {d}));
   return with_h || n == 0 ? 0 : run_shrink<T, true>(x, ldx, n, d, a, k, r, scales, s, s.h, st);
 }
 
@@ -1011,12 +1161,11 @@ template <typename T>
 int run_grads(Grad<T> g0, Grad<T> g1, int64_t n, int64_t k, int64_t r, const Save& s, int64_t per, hipStream_t st) {
   g0.blocks = (int)((g0.cols * (int64_t)sizeof(T) + 255) / 256);
   g1.blocks = (int)((g1.cols * (int64_t)sizeof(T) + 255) / 256);
-  const int64_t blocks = (int64_t)g0.blocks + g1.blocks, cols = (int64_t)g0.cols + g1.cols;
-  KGE_REQUIRE(blocks <= 65535);
+  const int64_t wgs = (n / per + k) * ((int64_t)g0.blocks + g1.blocks), cols = (int64_t)g0.cols + g1.cols;
+  KGE_REQUIRE(wgs < (int64_t)1 << 31);
   KGE_TRY(by_even<T>([&](auto even) -> int {
-    grads_kernel<T, even.value>
-        <<<dim3((unsigned)(n / per + k), (unsigned)blocks, (unsigned)(rank_pad(r) / 16)), dim3(256), 0, st>>>(
-            g0, g1, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per);
+    grads_kernel<T, even.value><<<dim3((unsigned)wgs, (unsigned)(rank_pad(r) / 16)), dim3(256), 0, st>>>(
+        g0, g1, (int)rank_pad(r), (int)k, (int)r, s.perm, s.start, (int)per);
     KGE_CHECK_LAUNCH();
     return 0;
   }, {g0.cols, g1.cols}));
@@ -1053,12 +1202,12 @@ int run_few(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t l
 // W^T [d, ldwt] and every A_t^T [d, r]: dx is the projection of dy by them
 template <typename T>
 int run_transpose(const T* w, int64_t ldw, int64_t m, int64_t d, const T* a, int64_t k, int64_t r, T* wt, int64_t ldwt, T* at,
-                  hipStream_t st) {
+                  const Save& s, hipStream_t st) {
   const int64_t across = (d + 31) / 32, w_tiles = across * ((m + 31) / 32), a_tiles = across * ((r + 31) / 32);
   KGE_REQUIRE(w_tiles + a_tiles * k < (int64_t)1 << 31);
   transpose_kernel<T><<<dim3((unsigned)(w_tiles + a_tiles * k)), dim3(256), 0, st>>>(
       Flip<T>{w, ldw, 0, (int)m, (int)d, wt, ldwt, 0}, Flip<T>{a, d, r * d, (int)r, (int)d, at, r, r * d}, (int)w_tiles,
-      (int)across, (int)a_tiles, (int)across);
+      (int)across, (int)a_tiles, (int)across, s.start);
   KGE_CHECK_LAUNCH();
   return 0;
 }
@@ -1115,7 +1264,7 @@ extern "C" int kge_adapter_backward(const void* dy, int dtype, int64_t lddy, int
     const T *dyt = (const T*)dy, *xt = (const T*)x, *wt = (const T*)w, *at = (const T*)a, *bt = (const T*)b;
     if (n > 0 && (dx || da)) KGE_TRY((run_shrink<T, false>(dyt, lddy, n, m, bt, k, r, scales, s, q.u, st)));
     if (n > 0 && dx) {
-      KGE_TRY(run_transpose<T>(wt, ldw, m, d, at, k, r, (T*)q.wt, q.ldwt, (T*)q.at, st));
+      KGE_TRY(run_transpose<T>(wt, ldw, m, d, at, k, r, (T*)q.wt, q.ldwt, (T*)q.at, s, st));
       KGE_TRY(run_project<T>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, (const T*)q.at, k, r, q.u, s, (T*)dx, lddx, st));
     }
     const Grad<T> ga{xt, ldx, (int)d, 0, q.u, (T*)da, 1, d, q.slabs_a}, gb{dyt, lddy, (int)m, 0, s.h, (T*)db, r, 1, q.slabs_b};

@@ -33,27 +33,25 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
-    """[rows, cols] whose rows start on 16 bytes."""
+    """[rows, cols] whose rows start on 16 bytes.  No view of a wider buffer: a Function's output that is a view
+    cannot be changed in place (known answers masked with -inf)."""
     per = 16 // like.element_size()
-    ld = (cols + per - 1) // per * per
-    buf = torch.empty(rows, ld, device=like.device, dtype=like.dtype)
-    return buf if ld == cols else buf[:, :cols]
+    return torch.empty_strided((rows, cols), ((cols + per - 1) // per * per, 1), device=like.device, dtype=like.dtype)
 
 
 def _forward(x, w, a, b, ids, scales, for_backward):
     """(y, what the backward pass needs)"""
     n, d = x.shape
     k, m, r = b.shape
-    per = 16 // x.element_size()
-    ld = (m + per - 1) // per * per  # rows of y start on 16 bytes
-    y = torch.empty(n, ld, device=x.device, dtype=x.dtype)
+    y = _padded(n, m, x)
     lib = L.lib()
     size = lib.kge_adapter_save_size(n, d, k, r)
     save = torch.empty(size, device=x.device, dtype=torch.uint8)
-    L._check(lib.kge_adapter_forward(x.data_ptr(), L.DTYPES[x.dtype], _ld(x), n, d, w.data_ptr(), _ld(w), m, a.data_ptr(),
-                                     b.data_ptr(), k, r, ids.data_ptr(), L.ptr(scales), y.data_ptr(), ld, save.data_ptr(),
-                                     size, for_backward, L.stream()), "kge_adapter_forward")
-    return y if ld == m else y[:, :m], save
+    L._check(lib.kge_adapter_forward(
+        x.data_ptr(), L.DTYPES[x.dtype], _ld(x), n, d, w.data_ptr(), _ld(w), m, a.data_ptr(), b.data_ptr(), k, r,
+        ids.data_ptr(), L.ptr(scales), y.data_ptr(), _ld(y), save.data_ptr(), size, for_backward, L.stream()),
+        "kge_adapter_forward")
+    return y, save
 
 
 class _AdaptedProjection(torch.autograd.Function):
@@ -91,8 +89,8 @@ def _as_they_are(x, w, a, b, ids, scales) -> bool:
     if L.CHECK_INDEX:
         return False
     dtype, dev, bs = x.dtype, x.get_device(), b.shape
-    if (dtype not in (torch.bfloat16, torch.float32) or w.dtype is not dtype or a.dtype is not dtype or b.dtype is not dtype
-            or len(bs) != 3 or w.get_device() != dev or a.get_device() != dev or b.get_device() != dev
+    if (dtype not in (torch.bfloat16, torch.float32) or w.dtype is not dtype or a.dtype is not dtype
+            or b.dtype is not dtype or len(bs) != 3 or w.get_device() != dev or a.get_device() != dev or b.get_device() != dev
             or ids.get_device() != dev or ids.dtype is not torch.int64):
         return False
     k, m, r = bs
@@ -103,8 +101,8 @@ def _as_they_are(x, w, a, b, ids, scales) -> bool:
                                    and scales.is_contiguous() and not scales.requires_grad):
         return False
     return (w.shape == (m, d) and a.shape == (k, r, d) and ids.shape == (n,) and min(d, m, k) >= 1 and 1 <= r <= MAX_RANK
-            and not w.requires_grad and x.is_contiguous() and w.is_contiguous() and a.is_contiguous() and b.is_contiguous()
-            and ids.is_contiguous())
+            and not w.requires_grad and x.is_contiguous() and w.is_contiguous() and a.is_contiguous()
+            and b.is_contiguous() and ids.is_contiguous())
 
 
 def _checked(x, w, a, b, ids, scales):
@@ -170,7 +168,8 @@ class LowRankAdapters(torch.nn.Module):
         if min(num_adapters, num_in, num_out) < 1 or not 1 <= rank <= MAX_RANK:
             raise ValueError(f"num_adapters={num_adapters}, rank={rank}, num_in={num_in}, num_out={num_out}: expected "
                              f"at least 1 each, ranks up to {MAX_RANK}")
-        self.a = torch.nn.Parameter(torch.randn(num_adapters, rank, num_in, device=device).mul_(num_in ** -0.5).to(dtype))
+        a = torch.randn(num_adapters, rank, num_in, device=device).mul_(num_in ** -0.5)
+        self.a = torch.nn.Parameter(a.to(dtype))
         self.b = torch.nn.Parameter(torch.zeros(num_adapters, num_out, rank, device=device, dtype=dtype))
         scale = 1.0 if alpha is None else float(alpha) / rank
         self.register_buffer("scales", torch.full((num_adapters,), scale, device=device, dtype=torch.float32))

@@ -75,3 +75,11 @@ def test_c_entries_refuse_bad_shapes_without_a_device():
             forward(save=None), forward(save=at + 4), forward(size=size - 1)} == {1001}
     assert lib.kge_adapter_backward(None, 0, 6, 4, 6, None, 8, 8, None, 8, None, None, 3, 2, None, at, size, None, 8, None,
                                     None, None, 0, None) == 1001
+
+
+def test_workspace_of_a_backward_pass_does_not_grow_with_the_adapters():
+    """Slabs are for adapters of more than 1024 rows, of which there are few however many adapters there are; only
+    the transposed adapters of dx take room for each (k r d elements)."""
+    size = lambda k, dx: L.lib().kge_adapter_backward_ws_size(0, 5000, 64, 1000, k, 8, dx, 1, 1)  # noqa: E731
+    assert size(100000, 0) <= size(10, 0)  # (u's partial sums: fewer with more adapters)
+    assert size(100000, 1) <= size(10, 1) + 100000 * 8 * 64 * 4

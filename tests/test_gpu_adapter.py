@@ -333,3 +333,62 @@ def test_post_training_run(engine):
     # the scores (|s| < 20) carry 2 (32 + 4) u |s|: 1e-4 of them through softmax slopes below 1 into gradients
     for p, g in ((a.grad, ga), (b.grad, gb)):
         assert float((p.cpu().double() - g).abs().max()) <= 1e-4 * max(1.0, float(g.abs().max()))
+
+
+def test_masked_in_place_before_the_backward_pass(engine):
+    """Known answers set to -inf in the result itself, whatever the alignment of its rows (m odd)."""
+    t, ids = inputs(40, 16, 51, 4, 3, torch.float32, 5)
+    a, b = (t[q].detach().requires_grad_(True) for q in ("a", "b"))
+    hide = torch.rand(40, 51, generator=torch.Generator().manual_seed(1)).cuda() < 0.2
+    y = engine.adapted_projection(t["x"], t["w"], a, b, ids, t["scales"])
+    masked = engine.adapted_projection(t["x"], t["w"], a, b, ids, t["scales"]).masked_fill_(hide, -float("inf"))
+    assert torch.equal(masked.detach(), y.detach().masked_fill(hide, -float("inf")))
+    got = torch.autograd.grad(masked, (a, b), t["dy"])
+    want = torch.autograd.grad(y, (a, b), t["dy"].masked_fill(hide, 0.0))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("n", [3, 40, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_infinite_request_gives_infinities_in_its_row(engine, n, dtype):
+    """W x and B h of a row with one infinity and zeros beside it, B and W of one sign each: inf, not NaN."""
+    d, m, r = 8, 24, 2
+    x = torch.zeros(n, d, dtype=dtype, device="cuda")
+    x[:, 0] = 1.0
+    x[1, 0] = float("inf")
+    w = torch.ones(m, d, dtype=dtype, device="cuda")
+    a = torch.ones(2, r, d, dtype=dtype, device="cuda")
+    b = torch.ones(2, m, r, dtype=dtype, device="cuda")
+    ids = (torch.arange(n, device="cuda") % 2)
+    y = engine.adapted_projection(x, w, a, b, ids)
+    rest = torch.arange(n, device="cuda") != 1
+    assert (y[1] == float("inf")).all() and (y[rest] == 3.0).all()
+
+
+@pytest.mark.parametrize("n, d, m, k, r, ids", [
+    (70001, 8, 12, 5, 2, "mixed"), (40000, 8, 8, 900, 1, "skewed"), (9000, 8, 9, 4100, 2, "mixed"),
+    (50, 24, 20, 40000, 3, "mixed")])
+def test_sorted_plan(engine, monkeypatch, n, d, m, k, r, ids):
+    """Many rows or many adapters: the order comes from a radix sort (of one digit, of two from 2046 adapters on)."""
+    t, i = inputs(n, d, m, k, r, torch.float32, n + k, ids)
+    want = reference(t, i, torch.float32)
+    got = run(engine, t, i)
+    for name in ("y", "dx", "da", "db"):
+        check(got[name], want[name], name)
+    again = run(engine, t, i)
+    assert all(torch.equal(again[name], got[name]) for name in got)
+    from kge import _lib as L
+    monkeypatch.setattr(L, "CHECK_INDEX", False)
+    bad = i.clone()
+    bad[1::7], bad[2::11] = k + 3, -5
+    out = (bad < -1) | (bad >= k)
+    y = run(engine, t, bad)["y"]
+    assert torch.isnan(y[out]).all() and torch.equal(y[~out], got["y"][~out])
+
+
+def test_gradients_beside_a_table_of_millions_of_rows(engine):
+    n, d, m, k, r = 3, 4, 4_300_007, 2, 1
+    t, i = inputs(n, d, m, k, r, torch.float32, 1, "all")
+    want, got = reference(t, i, torch.float32), run(engine, t, i)
+    for name in ("y", "dx", "da", "db"):
+        check(got[name], want[name], name)
