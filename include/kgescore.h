@@ -586,7 +586,8 @@ int kge_row_norm_max(const float* t, int64_t ldt, int64_t m, int d, float* out, 
 /* ---- losses on the log-probability of one label per score row -----------------------------------
  * Post-training of a trained model (no counterpart in the reference): score rows S [n, m] of type
  * dtype (KGE_DT_*), row stride lds in elements (any), labels[i] in [0, m) or -1 (the row carries
- * nothing: log-probability 0, zero gradient, not read).  x = S / temperature,
+ * nothing: log-probability 0, zero gradient, not read), n up to 2^30.  x = S / temperature, in
+ * [1e-30, 1e30],
  *   logp[i] = x[i, labels[i]] - logsumexp_j x[i, j]
  * A label outside [-1, m) gives NaN.  Needs a workspace of kge_label_ws_size bytes, 16-B aligned,
  * of this call's own (calls that overlap on the device must not share one); pairs: 0 except for
