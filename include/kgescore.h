@@ -636,12 +636,14 @@ int kge_preference_loss(const void* s, int dtype, int64_t lds, int64_t n, int64_
  * An id outside [-1, k) poisons its own row (NaN). */
 
 /* y [n, m].  save: kge_adapter_save_size bytes, 16-B aligned, of this call's own; for_backward 1: it holds the plan
- * and h afterwards, as kge_adapter_backward takes them.  scales null: 1. */
+ * and h afterwards, as kge_adapter_backward takes them.  ws: kge_adapter_forward_ws_size bytes (mostly 0: null), 16-B
+ * aligned, of this call's own.  scales null: 1. */
 int64_t kge_adapter_save_size(int64_t n, int64_t d, int64_t k, int64_t r);
+int64_t kge_adapter_forward_ws_size(int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r, int for_backward);
 int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
                         int64_t m, const void* a, const void* b, int64_t k, int64_t r, const int64_t* ids,
                         const float* scales, void* y, int64_t ldy, void* save, int64_t save_bytes, int for_backward,
-                        void* stream);
+                        void* ws, int64_t ws_bytes, void* stream);
 
 /* dx [n, d], da [k, r, d], db [k, m, r] for dy [n, m]; each may be null.  ws: kge_adapter_backward_ws_size bytes
  * (dx, da, db: whether that gradient is wanted), 16-B aligned, of this call's own. */

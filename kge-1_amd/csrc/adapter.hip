@@ -429,7 +429,8 @@ __global__ void __launch_bounds__(256) slabs_kernel(f32x4* __restrict__ x, int64
 // 1024 x 14541 x 512, bf16: 30 us without adapters (the traffic of W, x and y needs 9, the products 6), 47 us with 64
 // adapters of rank 16 (30 MB more); fp32: 159 us (96 TFLOP/s) and 172 us with 32 of rank 8.  Tried and slower: all of
 // x's rows of a workgroup in LDS with W straight into registers (32 / 50 us), a walk over tiles by as many workgroups
-// as fit (spills), slices straight into registers (33 / 49 us), twelve slices at a time (spills).
+// as fit (spills), slices straight into registers (33 / 49 us), sixteen slices at a time from the first stage on (31 /
+// 47 us), two stages on their way in registers (33 / 49 us): loads, LDS reads and products need 6 us each and take turns.
 constexpr int BN = 128, BKB = 128;  // rows of W (columns of y), bytes of the summed axis per stage
 
 // 16-byte slot of a 128-byte row, XOR-ed with the row: the 16 rows a fragment read touches then lie in
@@ -497,11 +498,14 @@ struct Piece {
 // BM 128: the tile above; BM 64: half of its rows, where 128-row tiles leave CUs without work.
 // bf16: three workgroups per CU (87 us against two's 92 at 1024 x 14541 x 2048); fragments of odd ranks need the
 // registers of two, or they spill.
-template <typename T, int BM, int STAGES, bool EVEN>
+// SPLIT: `per` elements of the summed axis per workgroup (blockIdx.y), the sums into slabs [split][n][m] of fp32, the
+// adapters into the first one's; split_join_kernel adds them up.
+template <typename T, int BM, int STAGES, bool EVEN, bool SPLIT>
 __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, const T* __restrict__ w, int64_t ldw, int m,
                    const T* __restrict__ f, int k, int r, int rp, const float* __restrict__ h, const int* __restrict__ perm,
-                   const int* __restrict__ sid, T* __restrict__ y, int64_t ldy, int row_tiles, int yvec) {
+                   const int* __restrict__ sid, T* __restrict__ y, int64_t ldy, int row_tiles, int yvec, int per,
+                   float* __restrict__ slabs) {
   constexpr int N = Mma<T>::N, KE = BKB / sizeof(T), KC = Mma<T>::KC;
   constexpr int XP = BM / 32, TM = BM / 32;  // pieces of x per thread and stage; 16-row fragments per wave
   constexpr int STAGE = (BM + BN) * BKB, LDS = STAGES * STAGE > 32768 ? STAGES * STAGE : 32768;
@@ -514,6 +518,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1;
   const int tile = xcd_remap(blockIdx.x, gridDim.x);
   const int m0 = (tile / row_tiles) * BN, n0 = (tile % row_tiles) * BM;
+  const int lo = SPLIT ? blockIdx.y * per : 0, hi = SPLIT ? min(d, lo + per) : d;
 
   const T* src[XP + 4];
   const int kt = (tid & 7) * N;  // first column of this thread's pieces within a stage
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
 #pragma unroll
     for (int j = 0; j < XP + 4; ++j) __builtin_memcpy(&reg[j], src[j] + k0, 16);
   };
-  if (KE <= d) load(0);
+  if (lo + KE <= hi) load(lo);
 
   // The tile's adapters: sorted rows, so each is a run; slot = its number within the tile (-1: no adapter).
   const int t_lo = n0 + lane < n ? sid[n0 + lane] : k;
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
   const uint64_t upto = lane == 63 ? ~0ull : (2ull << lane) - 1;
   const int slot_lo = t_lo < k ? __popcll(b_lo & upto) - 1 : -1;
   const int slot_hi = t_hi < k ? __popcll(b_lo) + __popcll(b_hi & upto) - 1 : -1;
-  const int slots = __popcll(b_lo) + __popcll(b_hi);
+  const int slots = SPLIT && blockIdx.y > 0 ? 0 : __popcll(b_lo) + __popcll(b_hi);
   if (wave == 0) {
     if ((b_lo >> lane) & 1) owner[slot_lo] = t_lo;
     if (BM == 128 && ((b_hi >> lane) & 1)) owner[slot_hi] = t_hi;
@@ -581,9 +586,9 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
   };
 
   int at = 0;  // the stage being filled
-  for (int k0 = 0; k0 < d; k0 += KE) {
-    if (STAGES == 1 && k0) __syncthreads();  // the stage has been read (of two, the barrier below has seen to it)
-    if (k0 + KE <= d) {
+  for (int k0 = lo; k0 < hi; k0 += KE) {
+    if (STAGES == 1 && k0 > lo) __syncthreads();  // the stage has been read (of two, the barrier below has seen to it)
+    if (k0 + KE <= hi) {
 #pragma unroll
       for (int j = 0; j < XP + 4; ++j)
         *reinterpret_cast<u32x4*>(&lds[at + lds_slot((tid >> 3) + j * 32, tid & 7)]) = reg[j];
@@ -591,13 +596,13 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
 #pragma unroll 1
       for (int row = tid >> 3; row < BM + BN; row += 32) {
         const T* p = row < BM ? x + (int64_t)perm[min(n0 + row, n - 1)] * ldx : w + (int64_t)min(m0 + row - BM, m - 1) * ldw;
-        *reinterpret_cast<u32x4*>(&lds[at + lds_slot(row, tid & 7)]) = frag<T, false>(p, k0 + kt, d);
+        *reinterpret_cast<u32x4*>(&lds[at + lds_slot(row, tid & 7)]) = frag<T, false>(p, k0 + kt, hi);
       }
     }
     __syncthreads();
-    if (k0 + 2 * KE <= d)
+    if (k0 + 2 * KE <= hi)
       load(k0 + KE);
-    else if (k0 + KE >= d)
+    else if (k0 + KE >= hi)
       fetch(0, 0);  // behind the last stage's products
 #pragma unroll
     for (int kc = 0; kc < KE / KC; ++kc) {
@@ -676,9 +681,16 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     const float poison = __shfl(mark, lane0 + i * 16 + fr, 64) == -2 ? NAN : 0.f;  // an id out of range
     if (n0 + wr * (BM / 2) + i * 16 + fr >= n) continue;
     T* yr = y + (int64_t)from[i] * ldy;
+    float* sr = SPLIT ? slabs + ((int64_t)blockIdx.y * n + from[i]) * m : nullptr;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = m0 + wc * 64 + j * 16 + fs * 4;
+      if (SPLIT) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < m) sr[c + e] = acc[i][j][e] + poison;
+        continue;
+      }
       typedef T out4 __attribute__((ext_vector_type(4)));
       out4 o;
 #pragma unroll
@@ -691,6 +703,18 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
           if (c + e < m) yr[c + e] = o[e];
       }
     }
+  }
+}
+
+// y = the slabs' sum, in their order
+template <typename T>
+__global__ void __launch_bounds__(256) split_join_kernel(const float* __restrict__ slabs, int64_t count, int splits, int m,
+                                                         T* __restrict__ y, int64_t ldy) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    float a = slabs[i];
+    for (int s = 1; s < splits; ++s) a += slabs[s * count + i];
+    const int64_t row = i / m;
+    y[row * ldy + (i - row * m)] = (T)a;
   }
 }
 
@@ -1040,8 +1064,11 @@ Save save_of(void* base, int64_t n, int64_t d, int64_t k, int64_t r) {
   return s;
 }
 
+int64_t split_ws(int64_t n, int64_t d, int64_t m, int es);
+
 struct BackWs {
   float* u;
+  float* splits;
   void *wt, *at;
   int64_t ldwt;
   int64_t per;
@@ -1060,6 +1087,8 @@ BackWs back_ws_of(void* base, int dtype, int64_t n, int64_t d, int64_t m, int64_
   if (dx) o += round256(d * s.ldwt * es);
   s.at = b + o;
   if (dx) o += round256(k * r * d * es);
+  s.splits = (float*)(b + o);
+  if (dx) o += split_ws(n, m, d, es);
   s.per = grads_per(n, (da ? d : 0) + (db ? m : 0), r, es);
   s.slabs_a = (float*)(b + o);
   if (da) o += grads_ws(n, d, r, s.per);
@@ -1130,31 +1159,60 @@ int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int
   return 0;
 }
 
+// Elements of the summed axis per workgroup of project (a multiple of a stage's; >= d: no split): where tiles leave
+// CUs idle, about two workgroups per CU with eight stages each at least; in fp32 no sum of more than 4096 products,
+// whose roundings would show (30000 products in one chain are off by 3e-6 of their size, in eight by 1e-6).
+int64_t split_per(int64_t n, int64_t d, int64_t m, int es) {
+  const int64_t stage = BKB / es, bn = (m + BN - 1) / BN;
+  int64_t tiles = ((n + 127) / 128) * bn;
+  if (tiles < PROJECT_SMALL * kge_num_cus()) tiles = ((n + 63) / 64) * bn;
+  const int64_t want = (2 * kge_num_cus() + tiles - 1) / std::max<int64_t>(1, tiles), most = std::max<int64_t>(1, d / (8 * stage));
+  int64_t splits = std::max<int64_t>(1, std::min(want, most));
+  if (es == 4) splits = std::max(splits, (d + 4095) / 4096);
+  return ((d + splits - 1) / splits + stage - 1) / stage * stage;
+}
+int64_t split_ws(int64_t n, int64_t d, int64_t m, int es) {
+  const int64_t per = split_per(n, d, m, es);
+  return per >= d ? 0 : round256((d + per - 1) / per * n * m * 4);
+}
+
 template <typename T, int BM>
 int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
-                   int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
+                   int64_t r, const float* h, const Save& s, T* y, int64_t ldy, float* slabs, hipStream_t st) {
   // fp32 is bound by its matrix instructions: two workgroups per CU with two stages each keep them fed, and
   // share the last round of tiles better than three (133 against 105 TFLOP/s at 4096^3)
   constexpr int STAGES = sizeof(T) == 4 ? 2 : 1;
   const int64_t row_tiles = (n + BM - 1) / BM, tiles = row_tiles * ((m + BN - 1) / BN);
-  KGE_REQUIRE(tiles < ((int64_t)1 << 31));
+  const int64_t per = split_per(n, d, m, sizeof(T)), splits = (d + per - 1) / per;
+  KGE_REQUIRE(tiles < ((int64_t)1 << 31) && splits <= 65535);
   const int yvec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T))) == 0 && ldy % 4 == 0;
-  return by_even<T>([&](auto even) -> int {
-    project_kernel<T, BM, STAGES, even.value><<<dim3((unsigned)tiles), dim3(256), 0, st>>>(
-        x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k, (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy,
-        (int)row_tiles, yvec);
+  KGE_TRY(by_even<T>([&](auto even) -> int {
+    auto launch = [&](auto kernel) {
+      kernel<<<dim3((unsigned)tiles, (unsigned)splits), dim3(256), 0, st>>>(
+          x, ldx, (int)n, (int)d, w, ldw, (int)m, f, (int)k, (int)r, (int)rank_pad(r), h, s.perm, s.sid, y, ldy,
+          (int)row_tiles, yvec, (int)per, slabs);
+    };
+    if (splits == 1)
+      launch(project_kernel<T, BM, STAGES, even.value, false>);
+    else
+      launch(project_kernel<T, BM, STAGES, even.value, true>);
     KGE_CHECK_LAUNCH();
     return 0;
-  }, {r});
+  }, {r}));
+  if (splits == 1) return 0;
+  split_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((n * m + 255) / 256, 8192)), dim3(256), 0, st>>>(
+      slabs, n * m, (int)splits, (int)m, y, ldy);
+  KGE_CHECK_LAUNCH();
+  return 0;
 }
 
 template <typename T>
 int run_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
-                int64_t r, const float* h, const Save& s, T* y, int64_t ldy, hipStream_t st) {
+                int64_t r, const float* h, const Save& s, T* y, int64_t ldy, float* slabs, hipStream_t st) {
   const int64_t tiles = ((n + 127) / 128) * ((m + BN - 1) / BN);
   return tiles < PROJECT_SMALL * kge_num_cus()
-             ? launch_project<T, 64>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st)
-             : launch_project<T, 128>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, st);
+             ? launch_project<T, 64>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, slabs, st)
+             : launch_project<T, 128>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, slabs, st);
 }
 
 template <typename T>
@@ -1218,13 +1276,20 @@ extern "C" int64_t kge_adapter_save_size(int64_t n, int64_t d, int64_t k, int64_
   return sizes_ok(KGE_DT_F32, n, d, 1, k, r) ? save_of(nullptr, n, d, k, r).bytes : 0;
 }
 
+extern "C" int64_t kge_adapter_forward_ws_size(int dtype, int64_t n, int64_t d, int64_t m, int64_t k, int64_t r,
+                                               int for_backward) {
+  return sizes_ok(dtype, n, d, m, k, r) && n > 0 && (for_backward || n > FEW) ? split_ws(n, d, m, elem_size(dtype)) : 0;
+}
+
 extern "C" int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_t n, int64_t d, const void* w, int64_t ldw,
                                    int64_t m, const void* a, const void* b, int64_t k, int64_t r, const int64_t* ids,
                                    const float* scales, void* y, int64_t ldy, void* save, int64_t save_bytes, int for_backward,
-                                   void* stream) {
+                                   void* ws, int64_t ws_bytes, void* stream) {
   KGE_REQUIRE(sizes_ok(dtype, n, d, m, k, r) && ld_ok(ldx, n, d) && ld_ok(ldw, m, d) && ld_ok(ldy, n, m));
   KGE_REQUIRE(save && aligned16(save) && save_bytes >= save_of(save, n, d, k, r).bytes);
   KGE_REQUIRE(n == 0 || (x && w && a && b && ids && y));
+  const int64_t ws_least = kge_adapter_forward_ws_size(dtype, n, d, m, k, r, for_backward);
+  KGE_REQUIRE(ws_bytes >= ws_least && (ws_least == 0 || (ws && aligned16(ws))));
   const Save s = save_of(save, n, d, k, r);
   const hipStream_t st = as_stream(stream);
   return by_type(dtype, [&](auto* tag) -> int {
@@ -1238,7 +1303,7 @@ extern "C" int kge_adapter_forward(const void* x, int dtype, int64_t ldx, int64_
     }
     KGE_TRY(run_plan_h<T>(ids, xt, ldx, n, d, at, k, r, scales, s, st));
     if (n == 0) return 0;
-    return run_project<T>(xt, ldx, n, d, wt, ldw, m, bt, k, r, s.h, s, yt, ldy, st);
+    return run_project<T>(xt, ldx, n, d, wt, ldw, m, bt, k, r, s.h, s, yt, ldy, (float*)ws, st);
   });
 }
 
@@ -1265,7 +1330,7 @@ extern "C" int kge_adapter_backward(const void* dy, int dtype, int64_t lddy, int
     if (n > 0 && (dx || da)) KGE_TRY((run_shrink<T, false>(dyt, lddy, n, m, bt, k, r, scales, s, q.u, st)));
     if (n > 0 && dx) {
       KGE_TRY(run_transpose<T>(wt, ldw, m, d, at, k, r, (T*)q.wt, q.ldwt, (T*)q.at, s, st));
-      KGE_TRY(run_project<T>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, (const T*)q.at, k, r, q.u, s, (T*)dx, lddx, st));
+      KGE_TRY(run_project<T>(dyt, lddy, n, m, (const T*)q.wt, q.ldwt, d, (const T*)q.at, k, r, q.u, s, (T*)dx, lddx, q.splits, st));
     }
     const Grad<T> ga{xt, ldx, (int)d, 0, q.u, (T*)da, 1, d, q.slabs_a}, gb{dyt, lddy, (int)m, 0, s.h, (T*)db, r, 1, q.slabs_b};
     const Grad<T> none{nullptr, 0, 0, 0, nullptr, nullptr, 0, 0, nullptr};

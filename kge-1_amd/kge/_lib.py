@@ -119,8 +119,9 @@ SIGNATURES = {
     "kge_preference_loss": ([_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _D, _D, _I, _D, _D, _P, _P, _P, _P, _P, _P,
                              _I64, _P, _I64, _P], _I),
     "kge_adapter_save_size": ([_I64, _I64, _I64, _I64], _I64),
+    "kge_adapter_forward_ws_size": ([_I, _I64, _I64, _I64, _I64, _I64, _I], _I64),
     "kge_adapter_forward": ([_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I,
-                             _P], _I),
+                             _P, _I64, _P], _I),
     "kge_adapter_backward_ws_size": ([_I, _I64, _I64, _I64, _I64, _I64, _I, _I, _I], _I64),
     "kge_adapter_backward": ([_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P,
                               _I64, _P, _P, _P, _I64, _P], _I),

@@ -44,12 +44,15 @@ def _forward(x, w, a, b, ids, scales, for_backward):
     n, d = x.shape
     k, m, r = b.shape
     y = _padded(n, m, x)
-    lib = L.lib()
+    lib, dtype = L.lib(), L.DTYPES[x.dtype]
     size = lib.kge_adapter_save_size(n, d, k, r)
     save = torch.empty(size, device=x.device, dtype=torch.uint8)
+    ws, ws_size = None, lib.kge_adapter_forward_ws_size(dtype, n, d, m, k, r, for_backward)
+    if ws_size:
+        ws = torch.empty(ws_size, device=x.device, dtype=torch.uint8)
     L._check(lib.kge_adapter_forward(
-        x.data_ptr(), L.DTYPES[x.dtype], _ld(x), n, d, w.data_ptr(), _ld(w), m, a.data_ptr(), b.data_ptr(), k, r,
-        ids.data_ptr(), L.ptr(scales), y.data_ptr(), _ld(y), save.data_ptr(), size, for_backward, L.stream()),
+        x.data_ptr(), dtype, _ld(x), n, d, w.data_ptr(), _ld(w), m, a.data_ptr(), b.data_ptr(), k, r, ids.data_ptr(),
+        L.ptr(scales), y.data_ptr(), _ld(y), save.data_ptr(), size, for_backward, L.ptr(ws), ws_size, L.stream()),
         "kge_adapter_forward")
     return y, save
 

@@ -68,7 +68,7 @@ def test_c_entries_refuse_bad_shapes_without_a_device():
 
     def forward(dtype=0, ldx=8, d=8, m=6, k=3, r=2, save=at, size=size):
         return lib.kge_adapter_forward(None, dtype, ldx, 4, d, None, 8, m, None, None, k, r, None, None, None, 6, save, size,
-                                       0, None)
+                                       0, None, 0, None)
 
     # null tensors, types, strides, sizes, workspaces: a status, never an exception
     assert {forward(), forward(dtype=2), forward(ldx=7), forward(m=0), forward(k=0), forward(r=1025),
@@ -83,3 +83,13 @@ def test_workspace_of_a_backward_pass_does_not_grow_with_the_adapters():
     size = lambda k, dx: L.lib().kge_adapter_backward_ws_size(0, 5000, 64, 1000, k, 8, dx, 1, 1)  # noqa: E731
     assert size(100000, 0) <= size(10, 0)  # (u's partial sums: fewer with more adapters)
     assert size(100000, 1) <= size(10, 1) + 100000 * 8 * 64 * 4
+
+
+def test_long_sums_of_few_rows_take_a_workspace():
+    """A sum of many products for few results is split over workgroups (slabs in fp32), forwards and for dx."""
+    forward = lambda *a: L.lib().kge_adapter_forward_ws_size(*a)  # noqa: E731
+    assert forward(0, 100, 40000, 64, 3, 4, 1) >= 2 * 100 * 64 * 4
+    assert forward(0, 20, 40000, 64, 3, 4, 0) == 0  # few requests: no tiles
+    assert forward(1, 1024, 512, 14541, 64, 16, 1) == 0 and forward(1, 0, 40000, 64, 3, 4, 1) == 0
+    back = lambda dx: L.lib().kge_adapter_backward_ws_size(0, 100, 64, 40000, 3, 4, dx, 0, 0)  # noqa: E731
+    assert back(1) >= back(0) + 2 * 100 * 64 * 4

@@ -392,3 +392,17 @@ def test_gradients_beside_a_table_of_millions_of_rows(engine):
     want, got = reference(t, i, torch.float32), run(engine, t, i)
     for name in ("y", "dx", "da", "db"):
         check(got[name], want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, d, m, k, r, ids", [
+    (100, 40, 20001, 5, 4, "mixed"), (70, 9000, 130, 3, 16, "mixed"), (33, 4100, 4100, 2, 1, "all"),
+    (200, 8192, 33, 4, 24, "none")])
+def test_split_sums(engine, n, d, m, k, r, ids, dtype):
+    """Few results of long sums: split over workgroups and joined, in dx (m long), forwards (d long) or both."""
+    t, i = inputs(n, d, m, k, r, dtype, n + d, ids, 3, 1)
+    want, got = reference(t, i, dtype), run(engine, t, i)
+    for name in ("y", "dx", "da", "db"):
+        check(got[name], want[name], name)
+    again = run(engine, t, i)
+    assert all(torch.equal(again[name], got[name]) for name in got)
