@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(256) slabs_kernel(f32x4* __restrict__ x, int64
 }
 
 // ---- project: y[perm[i], :] = W x + F_t h_i -----------------------------------------------------------
-// F_t as [m, r].  128 x 128 tiles, four waves of 64 x 64, one 32-KiB LDS stage of 128 bytes of the summed axis
+// F_t as [m, r].  128 x 128 tiles (rows of x, rows of W), four waves of 64 x 64, one 32-KiB LDS stage of 128 bytes of the summed axis
 // (fp32: two); the next stage waits in registers.  One stage instead of two lets three workgroups share a CU, whose
 // phases (loads, products, adapters, stores) overlap: with the short summed axes of embedding tables (512: 8 stages)
 // a bf16 tile is latency, not MFMA time.  The slices of eight adapters at a time come into registers behind the last
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(256) slabs_kernel(f32x4* __restrict__ x, int64
 // x's rows of a workgroup in LDS with W straight into registers (32 / 50 us), a walk over tiles by as many workgroups
 // as fit (spills), slices straight into registers (33 / 49 us), sixteen slices at a time from the first stage on (31 /
 // 47 us), two stages on their way in registers (33 / 49 us): loads, LDS reads and products need 6 us each and take turns.
-constexpr int BN = 128, BKB = 128;  // rows of W (columns of y), bytes of the summed axis per stage
+constexpr int BKB = 128;  // bytes of the summed axis per stage
 
 // 16-byte slot of a 128-byte row, XOR-ed with the row: the 16 rows a fragment read touches then lie in
 // eight different slots
@@ -458,8 +458,8 @@ __device__ __forceinline__ u32x4 h_frag<__bf16>(const float* h, int q0, int fs) 
   return __builtin_bit_cast(u32x4, o);
 }
 
-// Adapter slices in LDS: 16 ranks of 128 columns, [column][16 ranks].
-template <typename T>
+// Adapter slices in LDS: 16 ranks of BN columns, [column][16 ranks].
+template <typename T, int BN>
 struct Slice {
   static constexpr int ROW = 16 * sizeof(T), BYTES = BN * ROW;
   // where a lane's part of column `col` starts: the ranks its h fragment holds
@@ -480,10 +480,10 @@ __device__ __forceinline__ bool nonfinite(const u32x4& v, __bf16) {
   return b;
 }
 
-// A thread's 16-byte pieces of one slice: ranks [q0, q0 + 16) of columns [m0, m0 + 128) of an adapter.
-template <typename T, bool EVEN>
+// A thread's 16-byte pieces of one slice: ranks [q0, q0 + 16) of columns [m0, m0 + BN) of an adapter.
+template <typename T, int BN, bool EVEN>
 struct Piece {
-  static constexpr int N = Mma<T>::N, P = 16 / N, IT = BN * P / 256;  // pieces per column, per thread
+  static constexpr int N = Mma<T>::N, P = 16 / N, IT = (BN * P + 255) / 256;  // pieces per column, per thread
 
   static __device__ __forceinline__ u32x4 load(const T* ft, int m, int r, int m0, int q0, int it) {
     const int piece = it * 256 + threadIdx.x;
@@ -491,39 +491,42 @@ struct Piece {
   }
   static __device__ __forceinline__ void store(unsigned char* to, int it, const u32x4& v) {
     const int piece = it * 256 + threadIdx.x;
-    *reinterpret_cast<u32x4*>(to + piece / P * Slice<T>::ROW + piece % P * 16) = v;
+    if (piece < BN * P) *reinterpret_cast<u32x4*>(to + piece / P * Slice<T, BN>::ROW + piece % P * 16) = v;
   }
 };
 
 // BM 128: the tile above; BM 64: half of its rows, where 128-row tiles leave CUs without work.
 // bf16: three workgroups per CU (87 us against two's 92 at 1024 x 14541 x 2048); fragments of odd ranks need the
 // registers of two, or they spill.
+// BN 64: for at most 64 columns (dx of short queries), all four waves along the rows (a backward pass for dx of 4096 x 32
+// from 40000 columns in fp32: 461 us, 657 with tiles of 128).
 // SPLIT: `per` elements of the summed axis per workgroup (blockIdx.y), the sums into slabs [split][n][m] of fp32, the
 // adapters into the first one's; split_join_kernel adds them up.
-template <typename T, int BM, int STAGES, bool EVEN, bool SPLIT>
+template <typename T, int BM, int BN, int STAGES, bool EVEN, bool SPLIT>
 __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     project_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, const T* __restrict__ w, int64_t ldw, int m,
                    const T* __restrict__ f, int k, int r, int rp, const float* __restrict__ h, const int* __restrict__ perm,
                    const int* __restrict__ sid, T* __restrict__ y, int64_t ldy, int row_tiles, int yvec, int per,
                    float* __restrict__ slabs) {
   constexpr int N = Mma<T>::N, KE = BKB / sizeof(T), KC = Mma<T>::KC;
-  constexpr int XP = BM / 32, TM = BM / 32;  // pieces of x per thread and stage; 16-row fragments per wave
+  constexpr int WC = BN / 64, RW = BM * WC / 4, TM = RW / 16;  // waves along the columns; rows, 16-row fragments per wave
+  constexpr int XP = BM / 32, WP = BN / 32;  // pieces of x and of W per thread and stage
   constexpr int STAGE = (BM + BN) * BKB, LDS = STAGES * STAGE > 32768 ? STAGES * STAGE : 32768;
-  using PC = Piece<T, EVEN>;
+  using PC = Piece<T, BN, EVEN>;
   constexpr int COUNT = 8 / PC::IT;  // slices in LDS (and in registers, on their way) at a time: 32 KiB
-  static_assert(COUNT * Slice<T>::BYTES <= LDS, "slices");
+  static_assert(COUNT * Slice<T, BN>::BYTES <= LDS, "slices");
   __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
   __shared__ int owner[BM];
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fs = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WC, wc = wave % WC;
   const int tile = xcd_remap(blockIdx.x, gridDim.x);
   const int m0 = (tile / row_tiles) * BN, n0 = (tile % row_tiles) * BM;
   const int lo = SPLIT ? blockIdx.y * per : 0, hi = SPLIT ? min(d, lo + per) : d;
 
-  const T* src[XP + 4];
+  const T* src[XP + WP];
   const int kt = (tid & 7) * N;  // first column of this thread's pieces within a stage
 #pragma unroll
-  for (int j = 0; j < XP + 4; ++j) {
+  for (int j = 0; j < XP + WP; ++j) {
     const int row = (tid >> 3) + j * 32;
     if (j < XP)
       src[j] = x + (int64_t)perm[min(n0 + row, n - 1)] * ldx + kt;
@@ -533,7 +536,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
   u32x4 reg[8];
   auto load = [&](int k0) {  // a whole stage
 #pragma unroll
-    for (int j = 0; j < XP + 4; ++j) __builtin_memcpy(&reg[j], src[j] + k0, 16);
+    for (int j = 0; j < XP + WP; ++j) __builtin_memcpy(&reg[j], src[j] + k0, 16);
   };
   if (lo + KE <= hi) load(lo);
 
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     if (BM == 128 && ((b_hi >> lane) & 1)) owner[slot_hi] = t_hi;
   }
   // slot (or k + 1: an id out of range) of row `lane` of the half of the tile that this wave's rows lie in
-  const int half = BM == 128 ? wr : 0, lane0 = BM == 128 ? 0 : wr * 32;
+  const int half = wr * RW / 64, lane0 = wr * RW % 64;
   const int mark = (half ? t_hi : t_lo) > k ? -2 : (half ? slot_hi : slot_lo);
 
   f32x4 acc[TM][4];
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
 #pragma unroll
       for (int it = 0; it < PC::IT; ++it) {
         bad |= nonfinite(reg[s * PC::IT + it], T());
-        PC::store(lds + s * Slice<T>::BYTES, it, reg[s * PC::IT + it]);
+        PC::store(lds + s * Slice<T, BN>::BYTES, it, reg[s * PC::IT + it]);
       }
     }
     return bad;
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     if (STAGES == 1 && k0 > lo) __syncthreads();  // the stage has been read (of two, the barrier below has seen to it)
     if (k0 + KE <= hi) {
 #pragma unroll
-      for (int j = 0; j < XP + 4; ++j)
+      for (int j = 0; j < XP + WP; ++j)
         *reinterpret_cast<u32x4*>(&lds[at + lds_slot((tid >> 3) + j * 32, tid & 7)]) = reg[j];
     } else {  // the rest of the summed axis, zeros behind it
 #pragma unroll 1
@@ -612,7 +615,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
         wb[j] = *reinterpret_cast<const u32x4*>(&lds[at + lds_slot(BM + wc * 64 + j * 16 + fr, kc * 4 + fs)]);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const u32x4 xa = *reinterpret_cast<const u32x4*>(&lds[at + lds_slot(wr * (BM / 2) + i * 16 + fr, kc * 4 + fs)]);
+        const u32x4 xa = *reinterpret_cast<const u32x4*>(&lds[at + lds_slot(wr * RW + i * 16 + fr, kc * 4 + fs)]);
         if constexpr (sizeof(T) == 4) {  // the four instructions on one accumulator four apart
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -629,10 +632,10 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
     if (STAGES == 2) at = STAGE - at;
   }
 
-  // acc[i][j]: x row n0 + wr BM / 2 + i 16 + fr, columns m0 + wc 64 + j 16 + 4 fs + reg
+  // acc[i][j]: x row n0 + wr RW + i 16 + fr, columns m0 + wc 64 + j 16 + 4 fs + reg
   int from[TM];  // the rows' places in x, h and y
 #pragma unroll
-  for (int i = 0; i < TM; ++i) from[i] = perm[min(n0 + wr * (BM / 2) + i * 16 + fr, n - 1)];
+  for (int i = 0; i < TM; ++i) from[i] = perm[min(n0 + wr * RW + i * 16 + fr, n - 1)];
   u32x4 hf[TM];
   for (int q0 = 0, s0 = 0; slots > 0 && q0 < rp;) {
     if (s0 == 0)
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
       if (first < 0) continue;  // no adapter from this row on
       const int last = min(end < 0 ? slots - 1 : end, s_now + COUNT - 1);
       for (int s = max(first, s_now); s <= last; ++s) {
-        const unsigned char* sl = lds + (s - s_now) * Slice<T>::BYTES;
+        const unsigned char* sl = lds + (s - s_now) * Slice<T, BN>::BYTES;
         const bool own = si == s;
         u32x4 hm;
 #pragma unroll
@@ -663,12 +666,12 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
         if (!apart) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            Mma<T>::run(acc[i][j], *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
+            Mma<T>::run(acc[i][j], *reinterpret_cast<const u32x4*>(sl + Slice<T, BN>::at(wc * 64 + j * 16 + fr, fs)), hm);
         } else {  // an infinity times another row's 0 must not reach that row
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             f32x4 next = acc[i][j];  // the same sum in the same order for the adapter's own rows
-            Mma<T>::run(next, *reinterpret_cast<const u32x4*>(sl + Slice<T>::at(wc * 64 + j * 16 + fr, fs)), hm);
+            Mma<T>::run(next, *reinterpret_cast<const u32x4*>(sl + Slice<T, BN>::at(wc * 64 + j * 16 + fr, fs)), hm);
             if (own) acc[i][j] = next;
           }
         }
@@ -679,7 +682,7 @@ __global__ void __launch_bounds__(256, STAGES == 2 || !EVEN ? 2 : 3)
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const float poison = __shfl(mark, lane0 + i * 16 + fr, 64) == -2 ? NAN : 0.f;  // an id out of range
-    if (n0 + wr * (BM / 2) + i * 16 + fr >= n) continue;
+    if (n0 + wr * RW + i * 16 + fr >= n) continue;
     T* yr = y + (int64_t)from[i] * ldy;
     float* sr = SPLIT ? slabs + ((int64_t)blockIdx.y * n + from[i]) * m : nullptr;
 #pragma unroll
@@ -1161,11 +1164,13 @@ int run_shrink(const T* v, int64_t ldv, int64_t n, int64_t cols, const T* f, int
 
 // Elements of the summed axis per workgroup of project (a multiple of a stage's; >= d: no split): where tiles leave
 // CUs idle, about two workgroups per CU with eight stages each at least; in fp32 no sum of more than 4096 products,
-// whose roundings would show (30000 products in one chain are off by 3e-6 of their size, in eight by 1e-6).
+// whose roundings would show (in one chain dx from 30000 columns was off by 3e-6 of its norm, in eight or ten by
+// 1e-6).  A backward pass for dx of 100 x 64 from 40000 columns then takes 97 us in fp32, 68 in bf16.
+int64_t project_tiles(int64_t n, int64_t m, int64_t bm) { return (n + bm - 1) / bm * (m <= 64 ? 1 : (m + 127) / 128); }
 int64_t split_per(int64_t n, int64_t d, int64_t m, int es) {
-  const int64_t stage = BKB / es, bn = (m + BN - 1) / BN;
-  int64_t tiles = ((n + 127) / 128) * bn;
-  if (tiles < PROJECT_SMALL * kge_num_cus()) tiles = ((n + 63) / 64) * bn;
+  const int64_t stage = BKB / es;
+  int64_t tiles = project_tiles(n, m, 128);
+  if (tiles < PROJECT_SMALL * kge_num_cus()) tiles = project_tiles(n, m, 64);
   const int64_t want = (2 * kge_num_cus() + tiles - 1) / std::max<int64_t>(1, tiles), most = std::max<int64_t>(1, d / (8 * stage));
   int64_t splits = std::max<int64_t>(1, std::min(want, most));
   if (es == 4) splits = std::max(splits, (d + 4095) / 4096);
@@ -1176,13 +1181,13 @@ int64_t split_ws(int64_t n, int64_t d, int64_t m, int es) {
   return per >= d ? 0 : round256((d + per - 1) / per * n * m * 4);
 }
 
-template <typename T, int BM>
+template <typename T, int BM, int BN>
 int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
                    int64_t r, const float* h, const Save& s, T* y, int64_t ldy, float* slabs, hipStream_t st) {
   // fp32 is bound by its matrix instructions: two workgroups per CU with two stages each keep them fed, and
   // share the last round of tiles better than three (133 against 105 TFLOP/s at 4096^3)
   constexpr int STAGES = sizeof(T) == 4 ? 2 : 1;
-  const int64_t row_tiles = (n + BM - 1) / BM, tiles = row_tiles * ((m + BN - 1) / BN);
+  const int64_t row_tiles = (n + BM - 1) / BM, tiles = project_tiles(n, m, BM);
   const int64_t per = split_per(n, d, m, sizeof(T)), splits = (d + per - 1) / per;
   KGE_REQUIRE(tiles < ((int64_t)1 << 31) && splits <= 65535);
   const int yvec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T))) == 0 && ldy % 4 == 0;
@@ -1193,9 +1198,9 @@ int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, in
           (int)row_tiles, yvec, (int)per, slabs);
     };
     if (splits == 1)
-      launch(project_kernel<T, BM, STAGES, even.value, false>);
+      launch(project_kernel<T, BM, BN, STAGES, even.value, false>);
     else
-      launch(project_kernel<T, BM, STAGES, even.value, true>);
+      launch(project_kernel<T, BM, BN, STAGES, even.value, true>);
     KGE_CHECK_LAUNCH();
     return 0;
   }, {r}));
@@ -1209,10 +1214,10 @@ int launch_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, in
 template <typename T>
 int run_project(const T* x, int64_t ldx, int64_t n, int64_t d, const T* w, int64_t ldw, int64_t m, const T* f, int64_t k,
                 int64_t r, const float* h, const Save& s, T* y, int64_t ldy, float* slabs, hipStream_t st) {
-  const int64_t tiles = ((n + 127) / 128) * ((m + BN - 1) / BN);
-  return tiles < PROJECT_SMALL * kge_num_cus()
-             ? launch_project<T, 64>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, slabs, st)
-             : launch_project<T, 128>(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, slabs, st);
+  const bool short_tiles = project_tiles(n, m, 128) < PROJECT_SMALL * kge_num_cus();
+  const auto launch = m <= 64 ? (short_tiles ? launch_project<T, 64, 64> : launch_project<T, 128, 64>)
+                              : (short_tiles ? launch_project<T, 64, 128> : launch_project<T, 128, 128>);
+  return launch(x, ldx, n, d, w, ldw, m, f, k, r, h, s, y, ldy, slabs, st);
 }
 
 template <typename T>

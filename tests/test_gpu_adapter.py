@@ -406,3 +406,14 @@ def test_split_sums(engine, n, d, m, k, r, ids, dtype):
         check(got[name], want[name], name)
     again = run(engine, t, i)
     assert all(torch.equal(again[name], got[name]) for name in got)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, d, m, k, r, ids", [
+    (66000, 16, 20, 7, 8, "mixed"), (700, 64, 64, 30, 16, "skewed"), (150, 65, 63, 40, 20, "mixed")])
+def test_narrow_results(engine, n, d, m, k, r, ids, dtype):
+    """At most 64 columns of y or dx, in tiles of 128 rows and of 64."""
+    t, i = inputs(n, d, m, k, r, dtype, n + m, ids)
+    want, got = reference(t, i, dtype), run(engine, t, i)
+    for name in ("y", "dx", "da", "db"):
+        check(got[name], want[name], name)
