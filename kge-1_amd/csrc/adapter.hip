@@ -9,13 +9,14 @@
 //   u_i = scale_t B_t^T dy_i     dA_t = sum_{i in t} u_i x_i^T     dB_t = sum_{i in t} dy_i h_i^T
 //   dx_i = W^T dy_i + A_t^T u_i
 //
-// The rows are worked on in the order of their adapters (a stable counting sort of the ids: plan), so
-// that an adapter is read for 16 of its rows at a time; rows are gathered and scattered through the
-// order, never copied.  Four kernels:
+// The rows are worked on in the order of their adapters (plan: a stable counting sort of the ids, a radix sort
+// where there are many), so that an adapter is read for 16 of its rows at a time; rows are gathered and scattered
+// through the order, never copied.  After it:
 //   shrink   h (and u): [<= 16 rows of one adapter] x [d] x [r], the four waves of a workgroup split d
 //   project  W x + B h: a tiled product whose epilogue adds B_t h for every adapter among a fragment's 16
-//            rows.  Each adapter's product goes into accumulators of its own and is added to its own rows only:
-//            an adapter with infinities or NaN cannot reach another request's row.
+//            rows, h of the other rows masked to 0; a slice of B_t with infinities or NaN, whose products with 0
+//            would be NaN, is selected into its own rows instead: it cannot reach another request's row.  Long sums for
+//            few results are split over workgroups (split_join adds them up in order).
 //   grads    dA / dB: [r] x [rows of one adapter] x [columns] on the fp32 matrix instruction whatever the
 //            type (its operands hold one value per lane along the summed axis, so rows need no transpose)
 // h and u are kept in fp32; where they meet a bf16 B_t on the bf16 instruction they are split into hi + lo
@@ -822,9 +823,9 @@ __global__ void __launch_bounds__(256) project_few_kernel(const T* __restrict__ 
 // waves of a workgroup take every fourth group of four rows, GU groups on their way at once.  Adapters with more
 // than `per` rows are cut into chunks that write fp32 slabs, summed afterwards in ascending order.  An adapter without
 // rows gets zeros.  Both gradients (dA from x and u, dB from dy and h) in one launch.
-// fp32, 1024 x 14541 with 32 adapters of rank 8 of skewed sizes: 32 us for 77 MB (2.4 TB/s); its 7300 workgroups are
+// fp32, 1024 x 14541 with 32 adapters of rank 8 of skewed sizes: 30 us for 77 MB (2.6 TB/s); its 7300 workgroups are
 // short (the search of the chunk, the order, the rows, the sum over the waves, each waiting for the one before).
-// Several blocks of columns per workgroup: 27 to 22 us where adapters have equal shares, 32 to 37 with skewed ones.
+// Several blocks of columns per workgroup: 27 to 22 us where adapters have equal shares, 5 us more with skewed ones.
 template <typename T>
 struct Grad {
   const T* v;
