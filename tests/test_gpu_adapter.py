@@ -417,3 +417,31 @@ def test_narrow_results(engine, n, d, m, k, r, ids, dtype):
     want, got = reference(t, i, dtype), run(engine, t, i)
     for name in ("y", "dx", "da", "db"):
         check(got[name], want[name], name)
+
+
+@pytest.mark.parametrize("n, d, m, k, r", [(60000, 16, 12, 500, 2), (50, 40, 20001, 5, 4), (40, 9000, 30, 3, 3)])
+def test_sorted_plans_and_split_sums_recorded_in_a_graph(engine, n, d, m, k, r):
+    t, i = inputs(n, d, m, k, r, torch.float32, 1)
+
+    def work():
+        got = run(engine, t, i)
+        return [got[name].detach() for name in ("y", "dx", "da", "db")]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work()
+    for seed in range(3):
+        new, ids = inputs(n, d, m, k, r, torch.float32, 90 + seed, "skewed")
+        for name in t:
+            t[name].copy_(new[name])
+        i.copy_(ids)
+        want = [v.clone() for v in work()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
