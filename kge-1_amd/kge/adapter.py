@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
-from .label_losses import _capturing, on_device_of
+from .label_losses import _capturing, first_order, is_on_current_device, on_device_of
 
 MAX_RANK = 1024
 
@@ -36,7 +36,7 @@ def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """[rows, cols] whose rows start on 16 bytes.  No view of a wider buffer: a Function's output that is a view
     cannot be changed in place (known answers masked with -inf)."""
     per = 16 // like.element_size()
-    return torch.empty_strided((rows, cols), ((cols + per - 1) // per * per, 1), device=like.device, dtype=like.dtype)
+    return like.new_empty_strided((rows, cols), ((cols + per - 1) // per * per, 1))
 
 
 def _forward(x, w, a, b, ids, scales, for_backward):
@@ -64,26 +64,41 @@ class _AdaptedProjection(torch.autograd.Function):
         ctx.save_for_backward(x, w, a, b, scales, save)
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, dy):
-        x, w, a, b, scales, save = ctx.saved_tensors
-        n, d = x.shape
-        k, m, r = b.shape
-        want_x, _, want_a, want_b, _, _ = ctx.needs_input_grad
-        with on_device_of(x):
-            dy = _matrix(dy)
-            dx = _padded(n, d, x) if want_x else None
-            da = torch.empty_like(a) if want_a else None
-            db = torch.empty_like(b) if want_b else None
-            lib, dtype = L.lib(), L.DTYPES[x.dtype]
-            size = lib.kge_adapter_backward_ws_size(dtype, n, d, m, k, r, want_x, want_a, want_b)
-            ws = torch.empty(size, device=x.device, dtype=torch.uint8)
-            L._check(lib.kge_adapter_backward(
-                dy.data_ptr(), dtype, _ld(dy), n, m, x.data_ptr(), _ld(x), d, w.data_ptr(), _ld(w), a.data_ptr(),
-                b.data_ptr(), k, r, L.ptr(scales), save.data_ptr(), save.numel(), L.ptr(dx), _ld(dx) if want_x else d,
-                L.ptr(da), L.ptr(db), ws.data_ptr(), size, L.stream()), "kge_adapter_backward")
-        return dx, None, da, db, None, None
+        if not is_on_current_device(dy):
+            with torch.cuda.device(dy.get_device()):
+                return _gradients(ctx, dy)
+        return _gradients(ctx, dy)
+
+
+def _gradients(ctx, dy):
+    x, w, a, b, scales, save = ctx.saved_tensors
+    n, d = x.shape
+    k, m, r = b.shape
+    want_x, _, want_a, want_b, _, _ = ctx.needs_input_grad
+    dy = _matrix(dy)
+    dx, da, db = dx_at, da_at, db_at = None, None, None
+    ldx = d
+    if want_x:
+        dx = _padded(n, d, x)
+        dx_at, ldx = dx.data_ptr(), _ld(dx)
+    if want_a:
+        da = torch.empty_like(a)
+        da_at = da.data_ptr()
+    if want_b:
+        db = torch.empty_like(b)
+        db_at = db.data_ptr()
+    lib, dtype = L.lib(), L.DTYPES[x.dtype]
+    size = lib.kge_adapter_backward_ws_size(dtype, n, d, m, k, r, want_x, want_a, want_b)
+    ws = torch.empty(size, device=x.device, dtype=torch.uint8)
+    status = lib.kge_adapter_backward(
+        dy.data_ptr(), dtype, _ld(dy), n, m, x.data_ptr(), _ld(x), d, w.data_ptr(), _ld(w), a.data_ptr(), b.data_ptr(),
+        k, r, None if scales is None else scales.data_ptr(), save.data_ptr(), save.numel(), dx_at, ldx, da_at, db_at,
+        ws.data_ptr(), size, L.stream())
+    if status:
+        L._check(status, "kge_adapter_backward")
+    return dx, None, da, db, None, None
 
 
 def _as_they_are(x, w, a, b, ids, scales) -> bool:

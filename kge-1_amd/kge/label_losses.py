@@ -33,12 +33,13 @@ def _capturing() -> bool:
     return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
 
 
+def is_on_current_device(t: torch.Tensor) -> bool:
+    return _cur_device is not None and _cur_device() == t.get_device()
+
+
 def on_device_of(t: torch.Tensor):
     """A context in which t's device is the current one (launches go to ITS current stream)."""
-    dev = t.get_device()
-    if _cur_device is not None and _cur_device() == dev:
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    return contextlib.nullcontext() if is_on_current_device(t) else torch.cuda.device(t.get_device())
 
 
 def _score_rows(scores: torch.Tensor) -> torch.Tensor:
@@ -118,16 +119,19 @@ def _workspace(scores: torch.Tensor, pairs: int = 0):
     return torch.empty(size, device=scores.device, dtype=torch.uint8), size
 
 
+def _grad_ld(ld: int, m: int, scores: torch.Tensor) -> int:
+    if ld <= m + 64:
+        return ld
+    per = 16 // scores.element_size()
+    return (m + per - 1) // per * per
+
+
 def _grad_buffer(scores: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     """Where the gradient goes: ``out``, or new rows with the scores' stride (the kernels store 16
     bytes at a time where a row and its gradient are aligned alike), padded if that is far wider."""
     n, m = scores.shape
     if out is None:
-        ld = _ld(scores)
-        if ld > m + 64:
-            per = 16 // scores.element_size()
-            ld = (m + per - 1) // per * per
-        return torch.empty_strided((n, m), (ld, 1), device=scores.device, dtype=scores.dtype)
+        return scores.new_empty_strided((n, m), (_grad_ld(_ld(scores), m, scores), 1))
     if out.shape != scores.shape or out.dtype != scores.dtype or out.device != scores.device:
         raise ValueError("out: expected the scores' shape, type and device")
     if (m > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < m):
@@ -156,12 +160,31 @@ def _launch_logprobs(scores, labels, temperature, want_stats):
 
 
 def _launch_grad(scores, labels, temperature, stats, coef, gscale):
-    with on_device_of(scores):
-        grad = _grad_buffer(scores, None)
-        L._check(L.lib().kge_label_grad(L.ptr(scores), L.DTYPES[scores.dtype], _ld(scores), *scores.shape,
-                                        L.ptr(labels), temperature, L.ptr(stats), L.ptr(coef), L.ptr(gscale),
-                                        L.ptr(grad), _ld(grad), L.stream()), "kge_label_grad")
+    """(lean: it runs on autograd's device thread, where Python is slow and every launch-bound step waits for it)"""
+    if not is_on_current_device(scores):
+        with torch.cuda.device(scores.get_device()):
+            return _launch_grad(scores, labels, temperature, stats, coef, gscale)
+    n, m = scores.shape
+    ld = scores.stride(0) if n > 1 else m
+    ldg = _grad_ld(ld, m, scores)
+    grad = scores.new_empty_strided((n, m), (ldg, 1))
+    status = L.lib().kge_label_grad(scores.data_ptr(), L.DTYPES[scores.dtype], ld, n, m, labels.data_ptr(), temperature,
+                                    stats.data_ptr(), coef.data_ptr(), None if gscale is None else gscale.data_ptr(),
+                                    grad.data_ptr(), ldg, L.stream())
+    if status:
+        L._check(status, "kge_label_grad")
     return grad
+
+
+def first_order(gradient):
+    """The ``backward`` of a Function whose ``gradient(ctx, *grads)`` is no graph itself: once_differentiable, whose
+    wrapping only a pass that builds a graph (create_graph) pays for."""
+    once = torch.autograd.function.once_differentiable(gradient)
+
+    def backward(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else gradient(ctx, *grads)
+
+    return staticmethod(backward)
 
 
 class _LabelLogprobs(torch.autograd.Function):
@@ -172,8 +195,7 @@ class _LabelLogprobs(torch.autograd.Function):
         ctx.save_for_backward(scores, labels, stats)
         return logp
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, g):
         scores, labels, stats = ctx.saved_tensors
         return _launch_grad(scores, labels, ctx.temperature, stats, g.contiguous(), None), None, None
@@ -241,8 +263,7 @@ class _LabelLoss(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return loss, seen
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, g, _g_seen):
         if g is None:
             return None, None
