@@ -19,6 +19,7 @@ from . import _lib as L
 from .label_losses import _capturing, first_order, is_on_current_device, on_device_of
 
 MAX_RANK = 1024
+FEW = 32  # rows that take the path for few requests, which needs no workspace (the C entry has the same number)
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
@@ -47,9 +48,11 @@ def _forward(x, w, a, b, ids, scales, for_backward):
     lib, dtype = L.lib(), L.DTYPES[x.dtype]
     size = lib.kge_adapter_save_size(n, d, k, r)
     save = torch.empty(size, device=x.device, dtype=torch.uint8)
-    ws, ws_size = None, lib.kge_adapter_forward_ws_size(dtype, n, d, m, k, r, for_backward)
-    if ws_size:
-        ws = torch.empty(ws_size, device=x.device, dtype=torch.uint8)
+    ws, ws_size = None, 0
+    if for_backward or n > FEW:
+        ws_size = lib.kge_adapter_forward_ws_size(dtype, n, d, m, k, r, for_backward)
+        if ws_size:
+            ws = torch.empty(ws_size, device=x.device, dtype=torch.uint8)
     L._check(lib.kge_adapter_forward(
         x.data_ptr(), dtype, _ld(x), n, d, w.data_ptr(), _ld(w), m, a.data_ptr(), b.data_ptr(), k, r, ids.data_ptr(),
         L.ptr(scales), y.data_ptr(), _ld(y), save.data_ptr(), size, for_backward, L.ptr(ws), ws_size, L.stream()),

@@ -93,3 +93,9 @@ def test_long_sums_of_few_rows_take_a_workspace():
     assert forward(1, 1024, 512, 14541, 64, 16, 1) == 0 and forward(1, 0, 40000, 64, 3, 4, 1) == 0
     back = lambda dx: L.lib().kge_adapter_backward_ws_size(0, 100, 64, 40000, 3, 4, dx, 0, 0)  # noqa: E731
     assert back(1) >= back(0) + 2 * 100 * 64 * 4
+
+
+def test_few_requests_need_no_workspace():
+    from kge.adapter import FEW
+    for n in (FEW, FEW + 1):
+        assert (L.lib().kge_adapter_forward_ws_size(0, n, 40000, 64, 3, 4, 0) == 0) == (n == FEW)
