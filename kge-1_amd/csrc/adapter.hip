@@ -1034,7 +1034,7 @@ int64_t grads_ws(int64_t n, int64_t cols, int64_t r, int64_t per) {
 // (65536 rows of 237 adapters 46 us against 36 sorted, 2^20 rows 576 against 141, 8192 rows of 16000 adapters 142 against
 // 43; below: 32768 rows of 237 27 against 29 and three launches more, 8192 rows of 2000 32 against 54)
 constexpr int64_t SORT_FROM = 3 << 23;
-bool plan_sorted(int64_t n, int64_t k) { return std::max<int64_t>(n, 1024) * std::max<int64_t>(k + 2, 512) > SORT_FROM; }
+bool plan_sorted(int64_t n, int64_t k) { return n > 0 && std::max<int64_t>(n, 1024) * std::max<int64_t>(k + 2, 512) > SORT_FROM; }
 // rows of a wave: 512, or what leaves about 1024 waves
 int64_t sort_rows(int64_t n) { return std::max<int64_t>(512, (n + 1023) / 1024); }
 int64_t sort_bins(int64_t k) { return std::min<int64_t>(k + 2, BINS); }

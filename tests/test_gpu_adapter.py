@@ -445,3 +445,9 @@ def test_sorted_plans_and_split_sums_recorded_in_a_graph(engine, n, d, m, k, r):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_no_rows_beside_many_adapters(engine):
+    t, i = inputs(0, 4, 5, 30000, 1, torch.float32, 0)
+    got = run(engine, t, i)
+    assert got["y"].shape == (0, 5) and (got["da"] == 0).all() and (got["db"] == 0).all()
