@@ -78,7 +78,7 @@ def test_c_entries_refuse_bad_shapes_without_a_device():
 
 
 def test_workspace_of_a_backward_pass_does_not_grow_with_the_adapters():
-    """Slabs are for adapters of more than 1024 rows, of which there are few however many adapters there are; only
+    """Slabs are for adapters of more rows than a chunk, of which there are few however many adapters there are; only
     the transposed adapters of dx take room for each (k r d elements)."""
     size = lambda k, dx: L.lib().kge_adapter_backward_ws_size(0, 5000, 64, 1000, k, 8, dx, 1, 1)  # noqa: E731
     assert size(100000, 0) <= size(10, 0)  # (u's partial sums: fewer with more adapters)
